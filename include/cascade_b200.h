@@ -398,6 +398,118 @@ int32_t cb_owner_rank(const uint8_t *key, int32_t world);
 int cb_hash_batch_noalloc(int32_t device, const void *const *ptrs, const uint64_t *sizes, int32_t n,
                           uint8_t *digests_out, void *stream);
 
+/* ---- paged KV cache held in 4 bits --------------------------------------- */
+
+/* The operators a serving engine runs on a paged KV cache whose pages hold
+ * keys and values in 4 bits; no counterpart in the reference. They need no
+ * cb_store: pages are the caller's device memory, and a page is one block for
+ * cb_put_batch / cb_get_batch. All pointers below are DEVICE pointers on
+ * cache->device. Every call only enqueues work on `stream` (NULL = the legacy
+ * default stream), allocates nothing, never waits, and may be captured into a
+ * CUDA graph; calls on several streams need no order between them beyond that
+ * of the memory they share. Messages of failed calls are in
+ * cb_last_error(NULL). What only the device can see (a slot, page or length
+ * outside the cache) is skipped and sets CB_KV4_ERROR_RANGE in *errors.
+ *
+ * Format: x = offset + scale * (code - 8), one fp16 pair (scale, offset) per
+ * token, head and `group` dimensions. A (page, layer, head) is page_size/16
+ * tiles of [K codes 8*D][V codes 8*D][K params 64*D/group][V params
+ * 64*D/group] bytes (csrc/kv4.cuh gives the order inside). Values beyond
+ * +-65000 are stored as +-65000; a NaN makes its group NaN. */
+#define CB_KV4_F16 0
+#define CB_KV4_BF16 1
+#define CB_KV4_F32 2
+#define CB_KV4_ERROR_RANGE 1 /* bit of *errors: slot, page or length out of range */
+
+typedef struct cb_kv4_cache {
+  void *pages;          /* 16-byte aligned                                   */
+  uint64_t page_stride; /* bytes from page to page, a multiple of 16         */
+  uint32_t *errors;     /* error word, or NULL                               */
+  int32_t num_pages;
+  int32_t layers;       /* a page holds every layer: [layers][kv_heads][..]  */
+  int32_t kv_heads;
+  int32_t head_dim;     /* 64, 128 or 256                                    */
+  int32_t page_size;    /* tokens: 16, 32, 64, 128 or 256                    */
+  int32_t group;        /* 32, 64, 128 or 256, at most head_dim              */
+  int32_t device;
+  int32_t reserved32;
+} cb_kv4_cache;
+
+/* Bytes of a page (every layer and head), 0 for a form that is not offered. */
+uint64_t cb_kv4_page_bytes(int32_t layers, int32_t kv_heads, int32_t head_dim, int32_t page_size, int32_t group);
+
+/* Block tables, slots and positions of one step from request lengths.
+ * First every row with done[i] gives its pages [borrowed[i], pages held) back
+ * to the stack free[0 .. free_count) (rows and columns in order), and its length
+ * and borrowed count become 0. Then row i gets q_lens[i] new tokens (negative
+ * counts as 0): token j of row i is entry q_start[i] + j of slots (page *
+ * page_size + offset) and positions (kv_len + j). Missing pages come off the
+ * end of the stack, rows in order. A row is refused (status CB_PUT_FAILED, its
+ * slots -1, its length kept) if its tokens end past `tokens`, if they pass
+ * columns * page_size, or if it needs pages and the rows up to it need more
+ * than the stack has; a refused row's pages still count for the rows behind
+ * it. Entries behind the last token get slot -1, position 0. kv_lens_out
+ * and free_count_out may be kv_lens and free_count. */
+typedef struct cb_kv4_plan_args {
+  const int32_t *q_lens;
+  const uint8_t *done;   /* or NULL                                          */
+  const int32_t *kv_lens;
+  int32_t *kv_lens_out;
+  int32_t *borrowed;     /* leading pages of a row that are not its own      */
+  int32_t *block_table;  /* [requests][table_stride]                         */
+  int32_t *free;         /* [num_pages]                                      */
+  const int32_t *free_count;
+  int32_t *free_count_out;
+  int64_t *slots;        /* [tokens]                                         */
+  int32_t *positions;    /* [tokens]                                         */
+  int32_t *q_start;      /* [requests + 1]                                   */
+  uint8_t *status;       /* [requests]                                       */
+  uint32_t *errors;      /* or NULL                                          */
+  int64_t table_stride;
+  int32_t requests, columns, num_pages, page_size, tokens, device;
+} cb_kv4_plan_args;
+int cb_kv4_plan(const cb_kv4_plan_args *args, void *stream);
+
+/* Quantises n tokens' keys and values ([n][kv_heads][head_dim], strides in
+ * elements, head_dim contiguous) into the pages at their slots. Negative slots
+ * are skipped. A slot may appear once in a call. */
+int cb_kv4_append(const cb_kv4_cache *cache, int32_t layer, int32_t dtype, const void *k, const void *v, int32_t n,
+                  int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride,
+                  const int64_t *slots, void *stream);
+
+/* The inverse: tokens at `slots` as dense [n][kv_heads][head_dim] keys and
+ * values; zeros for a negative slot. */
+int cb_kv4_read(const cb_kv4_cache *cache, int32_t layer, int32_t dtype, void *k_out, void *v_out, int32_t n,
+                const int64_t *slots, void *stream);
+
+/* Attention of query rows over cached tokens. Request i has the rows
+ * q_start[i] .. q_start[i+1] (q_start NULL: one row each) of q
+ * [total_q][q_heads][head_dim] and the tokens 0 .. kv_lens[i] of its pages
+ * block_table[i][..]; row r of its n rows sees the tokens below kv_len - (n -
+ * 1 - r) when causal, else all of them. q_heads is a multiple of kv_heads. A
+ * row that sees nothing gets zeros and lse -inf. out: [total_q][q_heads]
+ * [head_dim] dense, of q's type; lse (natural log, [total_q][q_heads] fp32) or
+ * NULL. Rows behind q_start[requests] are left as they were. max_q is a hint
+ * (rows of a request at most); results do not depend on it being right.
+ * workspace: cb_kv4_attend_workspace bytes, 16-byte aligned, used until the
+ * call's work is done. */
+typedef struct cb_kv4_attend_args {
+  const void *q;
+  void *out;
+  float *lse;
+  const int32_t *block_table;
+  const int32_t *kv_lens;
+  const int32_t *q_start;
+  void *workspace;
+  uint64_t workspace_bytes;
+  int64_t table_stride;
+  int64_t q_token_stride, q_head_stride;
+  float scale; /* of q.k before the softmax */
+  int32_t layer, dtype, requests, columns, total_q, q_heads, max_q, causal, reserved32;
+} cb_kv4_attend_args;
+int cb_kv4_attend(const cb_kv4_cache *cache, const cb_kv4_attend_args *args, void *stream);
+uint64_t cb_kv4_attend_workspace(const cb_kv4_cache *cache, const cb_kv4_attend_args *args);
+
 #ifdef __cplusplus
 }
 #endif

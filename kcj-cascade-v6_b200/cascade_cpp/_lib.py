@@ -43,6 +43,11 @@ CB_FOUND_NOT_COPIED = 0x80
 
 CB_UID_BYTES = 128
 
+CB_KV4_F16 = 0
+CB_KV4_BF16 = 1
+CB_KV4_F32 = 2
+CB_KV4_ERROR_RANGE = 1
+
 
 class cb_config(C.Structure):
     _fields_ = [
@@ -100,6 +105,30 @@ class cb_location(C.Structure):
     ]
 
 
+class cb_kv4_cache(C.Structure):
+    _fields_ = [
+        ("pages", C.c_void_p), ("page_stride", C.c_uint64), ("errors", C.c_void_p),
+        ("num_pages", C.c_int32), ("layers", C.c_int32), ("kv_heads", C.c_int32), ("head_dim", C.c_int32),
+        ("page_size", C.c_int32), ("group", C.c_int32), ("device", C.c_int32), ("reserved32", C.c_int32),
+    ]
+
+
+class cb_kv4_plan_args(C.Structure):
+    _fields_ = [(f, C.c_void_p) for f in (
+        "q_lens", "done", "kv_lens", "kv_lens_out", "borrowed", "block_table", "free", "free_count",
+        "free_count_out", "slots", "positions", "q_start", "status", "errors")] + [
+        ("table_stride", C.c_int64)] + [(f, C.c_int32) for f in (
+            "requests", "columns", "num_pages", "page_size", "tokens", "device")]
+
+
+class cb_kv4_attend_args(C.Structure):
+    _fields_ = [(f, C.c_void_p) for f in (
+        "q", "out", "lse", "block_table", "kv_lens", "q_start", "workspace")] + [
+        ("workspace_bytes", C.c_uint64), ("table_stride", C.c_int64), ("q_token_stride", C.c_int64),
+        ("q_head_stride", C.c_int64), ("scale", C.c_float)] + [(f, C.c_int32) for f in (
+            "layer", "dtype", "requests", "columns", "total_q", "q_heads", "max_q", "causal", "reserved32")]
+
+
 # (name, restype, argtypes) — exactly the entry points of cascade_b200.h.
 _P = C.c_void_p
 _U8P = C.POINTER(C.c_uint8)
@@ -138,6 +167,13 @@ SIGNATURES = [
     ("cb_planner_create", C.c_int, [C.c_uint64, C.c_uint64, C.c_int32, C.c_int32, C.POINTER(_P)]),
     ("cb_planner_destroy", C.c_int, [_P]),
     ("cb_dht_plan_put", C.c_int, [_P, _P, _P, _P, C.c_int32, _P, _P]),
+    ("cb_kv4_page_bytes", C.c_uint64, [C.c_int32] * 5),
+    ("cb_kv4_plan", C.c_int, [C.POINTER(cb_kv4_plan_args), _P]),
+    ("cb_kv4_append", C.c_int, [C.POINTER(cb_kv4_cache), C.c_int32, C.c_int32, _P, _P, C.c_int32, C.c_int64,
+                                C.c_int64, C.c_int64, C.c_int64, _P, _P]),
+    ("cb_kv4_read", C.c_int, [C.POINTER(cb_kv4_cache), C.c_int32, C.c_int32, _P, _P, C.c_int32, _P, _P]),
+    ("cb_kv4_attend", C.c_int, [C.POINTER(cb_kv4_cache), C.POINTER(cb_kv4_attend_args), _P]),
+    ("cb_kv4_attend_workspace", C.c_uint64, [C.POINTER(cb_kv4_cache), C.POINTER(cb_kv4_attend_args)]),
 ]
 
 CB_NOALLOC_MAX_BLOCKS = 4096
