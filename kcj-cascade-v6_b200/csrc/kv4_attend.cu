@@ -4,11 +4,41 @@
 //   out = sum_t p_t v_t / sum_t p_t,  p_t = exp(scale * q.k_t - max)
 //
 // in one pass over a row's tokens with the running maximum and sum.
+#include <type_traits>
+
 #include "kv4.cuh"
 
 namespace cb {
 
 namespace {
+
+// Row tiles of 8*NT rows (query row x query head of one KV head), tokens in
+// tiles of 16. A unit of work is one token tile of one item (request, row tile,
+// KV head); the units of all items, in that order, are one long line, and every
+// CTA takes an equal piece of it, whatever the lengths are. An item that ends
+// up in several CTAs leaves partial sums in the workspace, joined by a second
+// kernel in a fixed order.
+//
+// Tensor-core form (16x8x16, fp16 in, fp32 sums): the cache is the 16-row
+// operand of both products and the 8*NT query rows the 8-wide one, so that the
+// at most 8 or 16 query heads of a KV head do not leave half of a product
+// empty:
+//   S[token][row]  = K[token][dim] . Q[dim][row]
+//   O[dim][row]   += V[dim][token] . P[token][row]
+// Both operands of the cache are raw codes: a nibble under a mask is the fp16
+// subnormal code * 2^-24 (second nibble: * 2^-20, undone in Q, or in O's rows),
+// exact, with no conversion. Scales and offsets act on 16x8 scores instead of
+// 16xD values: s = scale_k (q.c) + (offset_k - 8 scale_k) sum(q), and V's scale
+// goes into P, p' = p * scale_v, its offset into a sum of p * offset_v - 8 p'.
+// So the only roundings to 16 bits are p' (relative 2^-11; its rounded value
+// is the one that the centring by 8 uses) and the output. q is brought to fp16
+// by a power of two per row: exact for fp16 and, above 2^-28 of the row's
+// largest, for bf16.
+constexpr int kWarps = 8, kThreads = kWarps * 32;
+constexpr int kRecentre = 8;      // tiles between centrings of the sums
+constexpr float kSlack = 8.0f;    // p may reach 2^8 before the maximum is raised
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr uint32_t kWaitLimit = 1u << 24;
 
 struct AttendArgs {
   const void *q;
@@ -16,107 +46,776 @@ struct AttendArgs {
   float *lse;
   const int32_t *block_table, *kv_lens, *q_start;
   int64_t table_stride, q_token_stride, q_head_stride;
+  float *parts;  // partial sums: two per CTA
+  int4 *joins;   // per CTA: (first row tile entry, parts) of an item it begins and does not end
   float scale;
-  int32_t requests, columns, total_q, q_heads, causal, group;
+  int32_t requests, columns, total_q, q_heads, ratio, causal, bf16, min_share;
 };
 
-// The rows [q0, q1) of request r, inside [0, total_q).
-CB_D void request_rows(const AttendArgs &a, int r, int &q0, int &q1) {
-  if (!a.q_start) {
-    q0 = r;
-    q1 = r + 1;
-  } else {
-    q0 = min(max(a.q_start[r], 0), a.total_q);
-    q1 = min(max(a.q_start[r + 1], q0), a.total_q);
+// What an item is: request b, row tile rt, KV head h, and its token tiles.
+struct Item {
+  int b, rt, h;
+  int q0, qn, len;  // the request's rows and tokens
+  int tiles;        // at least 1: a row tile that sees nothing still writes zeros
+};
+
+template <int D, int NG, int NT>
+struct Form {
+  static constexpr int kRows = 8 * NT;
+  static constexpr int kTile = 16 * D + 128 * NG;   // bytes
+  static constexpr int kSlabs = D > 128 ? 2 : 1;
+  static constexpr int kWpr = D / kSlabs / 32;      // words a lane reads of a row and slab
+  static constexpr int kWords = D / 32;
+  static constexpr int kGroupWords = kWords / NG;
+  // bytes in flight: 8 or 16 warps with 4 tiles of 1.2 - 2.6 KB are 70 KB and more on
+  // an SM; HBM needs about 6.5 TB/s * 0.8 us / 148 = 35 KB
+  static constexpr int kStages = D > 128 || NG > 2 ? 3 : 4;
+  static constexpr int kCtasPerSm = NT == 1 && D <= 128 ? 2 : 1;
+  static constexpr bool kQRegs = NT == 1 && D <= 128;
+  static constexpr int kOutStride = D + 4;          // two rows are 8 banks apart
+  static constexpr int kRing = kWarps * kStages * kTile;
+  static constexpr int kQ = NT * (D / 16) * 32 * 8;
+  static constexpr int kConst = kRows * (2 + NG) * 4;
+  static constexpr int kMerge = kWarps * 8 * (kOutStride + 2) * 4;
+  static constexpr int kSmem = kRing + kQ + kMerge + kConst + kWarps * kStages * 8 + 128;
+  static constexpr int kPart = kRows * (D + 2);     // floats of a partial result
+};
+
+CB_D uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+CB_D void bar_init(uint32_t bar, uint32_t n) { asm volatile("mbarrier.init.shared.b64 [%0], %1;" ::"r"(bar), "r"(n)); }
+
+CB_D bool bar_wait(uint32_t bar, uint32_t parity) {
+  for (uint32_t i = 0; i < kWaitLimit; ++i) {
+    uint32_t ok;
+    asm volatile(
+        "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (ok) return true;
+  }
+  return false;
+}
+
+CB_D void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
+  asm volatile("mbarrier.arrive.expect_tx.shared.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+
+CB_D void mma(float *c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+CB_D uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+CB_D float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+template <int N>
+CB_D void load_words(const uint8_t *p, uint32_t *w) {
+  if constexpr (N == 1) w[0] = *reinterpret_cast<const uint32_t *>(p);
+  if constexpr (N == 2) {
+    const uint2 v = *reinterpret_cast<const uint2 *>(p);
+    w[0] = v.x, w[1] = v.y;
+  }
+  if constexpr (N >= 4) {
+#pragma unroll
+    for (int i = 0; i < N / 4; ++i) {
+      const uint4 v = *reinterpret_cast<const uint4 *>(p + 16 * i);
+      w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
+    }
   }
 }
 
-// One warp per (row, head): 32 tokens at a time, a lane for each while scores
-// are taken, then a share of the dimensions for each while values are summed.
-template <typename T, int D>
-__global__ void __launch_bounds__(128) attend_kernel(const Kv4View c, const AttendArgs a) {
-  constexpr int kWords = (D < 128 ? D : 128) / 32, kMine = D / 32;
-  const int lane = threadIdx.x & 31;
-  const int64_t id = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int row = (int)(id / a.q_heads), head = (int)(id % a.q_heads);
-  if (row >= a.total_q) return;
-  int r = 0, q0 = 0, q1 = 0;
-  for (; r < a.requests; ++r) {
-    request_rows(a, r, q0, q1);
-    if (row >= q0 && row < q1) break;
+// The rows [q0, q0 + qn) of request b, inside [0, total_q), and its tokens.
+CB_D void load_request(const AttendArgs &a, int most, int b, int &q0, int &qn, int &len) {
+  if (!a.q_start) {
+    q0 = b;
+    qn = 1;
+  } else {
+    q0 = min(max(__ldg(a.q_start + b), 0), a.total_q);
+    qn = min(max(__ldg(a.q_start + b + 1), q0), a.total_q) - q0;
   }
-  if (r == a.requests) return;
-  const int kvh = head / (a.q_heads / c.kv_heads), ng = D / a.group;
-  const int64_t most = (int64_t)a.columns * c.page_size;
-  int64_t len = a.kv_lens[r];
-  if (len < 0 || len > most) {
-    kv4_error(c.errors, kErrBounds);
-    len = len < 0 ? 0 : most;
+  len = min(max(__ldg(a.kv_lens + b), 0), most);
+}
+
+// Tokens that row r (of qn * ratio) of a request sees.
+CB_D int row_limit(const AttendArgs &a, const Item &it, int r) {
+  return a.causal ? it.len - (it.qn - 1 - r / a.ratio) : it.len;
+}
+
+template <int ROWS>
+CB_D void item_tiles(const AttendArgs &a, Item &it) {
+  const int last = min((it.rt + 1) * ROWS, it.qn * a.ratio) - 1;
+  it.tiles = max(1, (row_limit(a, it, last) + kKv4Tile - 1) / kKv4Tile);
+}
+
+// Tiles of all items of request b.
+template <int ROWS>
+CB_D long long request_tiles(const AttendArgs &a, int heads, int most, int b) {
+  Item it;
+  load_request(a, most, b, it.q0, it.qn, it.len);
+  long long n = 0;
+  const int rts = (it.qn * a.ratio + ROWS - 1) / ROWS;
+  for (it.rt = 0; it.rt < rts; ++it.rt) {
+    item_tiles<ROWS>(a, it);
+    n += it.tiles;
   }
-  const int64_t limit = a.causal ? len - (q1 - 1 - row) : len;
-  const T *q = static_cast<const T *>(a.q) + row * a.q_token_stride + head * a.q_head_stride;
-  float m = -INFINITY, l = 0.0f, o[kMine];
+  return n * heads;
+}
+
+// The item behind `it`; false behind the last.
+template <int ROWS>
+CB_D bool next_item(const AttendArgs &a, int heads, int most, Item &it) {
+  if (++it.h < heads) return true;
+  it.h = 0;
+  ++it.rt;
+  while (it.rt * ROWS >= it.qn * a.ratio) {
+    it.rt = 0;
+    if (++it.b >= a.requests) return false;
+    load_request(a, most, it.b, it.q0, it.qn, it.len);
+  }
+  item_tiles<ROWS>(a, it);
+  return true;
+}
+
+CB_D long long warp_sum(long long x) {
 #pragma unroll
-  for (int i = 0; i < kMine; ++i) o[i] = 0.0f;
-  for (int64_t t0 = 0; t0 < limit; t0 += 32) {
-    const int64_t pos = t0 + lane;
-    const uint8_t *tile = nullptr;
-    if (pos < limit) {
-      const int page = a.block_table[r * a.table_stride + (pos >> c.page_log2)];
-      if (page >= 0 && page < c.num_pages)
-        tile = c.base + page * c.page_stride + kvh * c.head_bytes +
-               (uint64_t)((pos & (c.page_size - 1)) / kKv4Tile) * kv4_tile_bytes(D, a.group);
-      else
-        kv4_error(c.errors, kErrBounds);
+  for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
+}
+
+// Finds this CTA's piece [f0, f1) of the line of units and the item that holds
+// f0 (its first unit is `first`). All threads return the same.
+template <int ROWS>
+CB_D bool find_piece(const AttendArgs &a, const Kv4View &c, int most, long long &share, long long &f0, long long &f1,
+                     long long &first, Item &it) {
+  __shared__ long long sums[kWarps], at_s;
+  __shared__ int where;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  long long total = 0, mine = 0;
+  for (int b = threadIdx.x; b < a.requests; b += kThreads) {
+    mine = request_tiles<ROWS>(a, c.kv_heads, most, b);
+    total += mine;
+    const int len = __ldg(a.kv_lens + b);
+    if (blockIdx.x == 0 && (len < 0 || len > most)) kv4_error(c.errors, kErrBounds);
+  }
+  total = warp_sum(total);
+  if (lane == 0) sums[warp] = total;
+  if (threadIdx.x == 0) where = -1;
+  __syncthreads();
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) total += sums[w];
+  share = max((total + gridDim.x - 1) / gridDim.x, (long long)a.min_share);
+  f0 = blockIdx.x * share;
+  f1 = min(f0 + share, total);
+  if (f0 >= f1) return false;
+  long long before = 0;
+  for (int b0 = 0; b0 < a.requests; b0 += kThreads) {
+    const int b = b0 + threadIdx.x;
+    if (a.requests > kThreads) mine = b < a.requests ? request_tiles<ROWS>(a, c.kv_heads, most, b) : 0;
+    else if (b >= a.requests) mine = 0;
+    long long v = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += y;
     }
-    const int tok = (int)(pos % kKv4Tile);
-    float s = -INFINITY;
-    if (tile) {
-      s = 0.0f;
-      const uint32_t *kw = reinterpret_cast<const uint32_t *>(tile);
-      const uint32_t *par = reinterpret_cast<const uint32_t *>(tile + 16 * D) + tok * ng;
-      for (int d = 0; d < D; ++d) {
-        const int slab = d / 128, x = d % 128, i = x / 32, t = x % 32 / 8, n = x % 8;
-        const uint32_t w = kw[((slab * 16 + tok) * 4 + t) * kWords + i];
-        const uint32_t pr = par[d / a.group];
-        s = fmaf(kv4_load1(q + d), kv4_value(w >> (4 * ((n & 1) * 4 + n / 2)) & 15u, kv4_scale(pr), kv4_offset(pr)), s);
+    __syncthreads();
+    if (lane == 31) sums[warp] = v;
+    __syncthreads();
+    long long chunk = 0, at = before + v - mine;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) at += sums[w];
+      chunk += sums[w];
+    }
+    if (at <= f0 && f0 < at + mine) {
+      where = b;
+      at_s = at;
+    }
+    before += chunk;
+    if (before > f0) break;  // the same for all threads
+  }
+  __syncthreads();
+  it.b = where;
+  first = at_s;
+  load_request(a, most, it.b, it.q0, it.qn, it.len);
+  for (it.rt = 0;; ++it.rt) {
+    item_tiles<ROWS>(a, it);
+    const long long n = (long long)it.tiles * c.kv_heads;
+    if (f0 < first + n) break;
+    first += n;
+  }
+  it.h = (int)((f0 - first) / it.tiles);
+  first += (long long)it.h * it.tiles;
+  return true;
+}
+
+template <int D, int NG, int NT>
+__global__ void __launch_bounds__(kThreads, Form<D, NG, NT>::kCtasPerSm)
+    attend_few_kernel(const Kv4View c, const AttendArgs a) {
+  using F = Form<D, NG, NT>;
+  extern __shared__ uint8_t raw[];
+  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 127) & ~(uintptr_t)127);
+  uint32_t *qs = reinterpret_cast<uint32_t *>(smem + F::kRing);
+  float *merge = reinterpret_cast<float *>(smem + F::kRing + F::kQ);
+  float *merge_ml = merge + kWarps * 8 * F::kOutStride;
+  float *q_scale = reinterpret_cast<float *>(smem + F::kRing + F::kQ + F::kMerge);
+  int *limits = reinterpret_cast<int *>(q_scale + F::kRows);
+  float *q_sum = reinterpret_cast<float *>(limits + F::kRows);  // [NG][rows]
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  uint8_t *ring = smem + warp * F::kStages * F::kTile;
+  const uint32_t bars =
+      smem_addr(smem + F::kRing + F::kQ + F::kMerge + F::kConst) + (uint32_t)warp * F::kStages * 8;
+  const int most = (int)min((long long)a.columns * c.page_size, 0x7fffffffll);
+  const int per_page = c.page_log2 - 4;
+
+  asm volatile("griddepcontrol.launch_dependents;");
+  if (lane == 0) {
+    for (int i = 0; i < F::kStages; ++i) bar_init(bars + 8 * i, 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  __syncwarp();
+  long long share, f0, f1, first;
+  Item it;
+  if (!find_piece<F::kRows>(a, c, most, share, f0, f1, first, it)) {
+    if (threadIdx.x == 0) a.joins[blockIdx.x] = make_int4(0, 0, 0, 0);
+    return;
+  }
+
+  // The warp's units are f0 + warp + 8 i. `ahead` runs kStages of them before
+  // the products, with the page of its next unit already asked for.
+  Item ahead = it;
+  long long a_unit = f0 + warp, a_first = first;
+  int a_page = -1;
+  bool a_there = a_unit < f1;
+  uint32_t held = 0, parity = 0;  // a bit for each stage: has data; wait parity
+  auto ahead_find = [&]() {  // moves to the item of a_unit and asks for its page
+    a_there = a_unit < f1;
+    while (a_there && a_unit >= a_first + ahead.tiles) {
+      a_first += ahead.tiles;
+      a_there = next_item<F::kRows>(a, c.kv_heads, most, ahead);
+    }
+    if (a_there) {
+      const int tile = (int)(a_unit - a_first);
+      a_page = tile * kKv4Tile < ahead.len
+                   ? __ldg(a.block_table + ahead.b * a.table_stride + (tile >> per_page))
+                   : -2;  // a row tile that sees nothing
+    }
+  };
+  auto ahead_issue = [&](int stage) {
+    held &= ~(1u << stage);
+    if (!a_there) return;
+    if (a_page >= 0 && a_page < c.num_pages) {
+      held |= 1u << stage;
+      if (lane == 0) {
+        const int tile = (int)(a_unit - a_first);
+        bulk_load(smem_addr(ring + stage * F::kTile),
+                  c.base + (uint64_t)a_page * c.page_stride + (uint64_t)ahead.h * c.head_bytes +
+                      (uint64_t)(tile & ((1 << per_page) - 1)) * F::kTile,
+                  F::kTile, bars + 8 * stage);
       }
-      s *= a.scale * 1.4426950408889634f;
+    } else if (a_page != -2 && lane == 0) {
+      kv4_error(c.errors, kErrBounds);
     }
-    float top = s;
-    for (int x = 16; x; x >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, x));
-    // a NaN score makes the row NaN (fmaxf drops it)
-    const float m2 = __any_sync(0xffffffffu, s != s) ? NAN : fmaxf(m, top);
-    if (m2 == -INFINITY) continue;
-    const float f = exp2f(m - m2);
-    const float p = tile ? exp2f(s - m2) : 0.0f;
-    m = m2;
-    l = l * f + p;
+    a_unit += kWarps;
+    ahead_find();
+  };
+  ahead_find();
+#pragma unroll 1
+  for (int i = 0; i < F::kStages; ++i) ahead_issue(i);
+
+  int stage = 0;
+  long long unit = f0 + warp;
+  int4 join = make_int4(0, 0, 0, 0);
+  bool first_segment = true;
+  for (long long seg = f0; seg < f1;) {
+    const long long end = min(first + it.tiles, f1);  // of this segment
+    const int rows = min(F::kRows, it.qn * a.ratio - it.rt * F::kRows);
+    // ---- the query rows: fp16 operands, their scale, their sums by group
+#pragma unroll 1
+    for (int r = warp; r < F::kRows; r += kWarps) {
+      constexpr int kMine = D / 32;
+      float x[kMine];
+      float top = 0.0f;
+      const int row = it.rt * F::kRows + r;
+      if (r < rows) {
+        const int64_t at = (int64_t)(it.q0 + row / a.ratio) * a.q_token_stride +
+                           (int64_t)(it.h * a.ratio + row % a.ratio) * a.q_head_stride + lane * kMine;
 #pragma unroll
-    for (int i = 0; i < kMine; ++i) o[i] *= f;
-    for (int j = 0; j < 32; ++j) {
-      const float pj = __shfl_sync(0xffffffffu, p, j);
-      const uint64_t at = __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(tile), j);
-      if (!at) continue;
-      const int tj = (int)((t0 + j) % kKv4Tile);
-      const uint16_t *vw = reinterpret_cast<const uint16_t *>(at + 8 * D);
-      const uint32_t *par = reinterpret_cast<const uint32_t *>(at + 16 * D + 64 * ng) + tj * ng;
+        for (int i = 0; i < kMine; ++i) {
+          x[i] = a.bf16 ? kv4_load1(static_cast<const __nv_bfloat16 *>(a.q) + at + i)
+                        : kv4_load1(static_cast<const __half *>(a.q) + at + i);
+          top = fmaxf(top, fabsf(x[i]));
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < kMine; ++i) x[i] = 0.0f;
+      }
+      float sum = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) sum += x[i];
+      for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      for (int o = 1; o < 32 / NG; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      // 2^(14 - e) with e the exponent of the largest; powers of two are exact
+      const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 110);
+      const float up = __uint_as_float((uint32_t)(14 - e + 127) << 23);
 #pragma unroll
       for (int i = 0; i < kMine; ++i) {
-        const int d = i * 32 + lane, slab = d / 128, x = d % 128;
-        const uint32_t w = vw[((((slab * 2 + tj / 8) * 8 + x % 8) * 4 + tj % 8 / 2) * kWords + x / 32) * 2 + tj % 2];
-        const uint32_t pr = par[d / a.group];
-        o[i] = fmaf(pj, kv4_value(w >> (4 * (x % 32 / 8)) & 15u, kv4_scale(pr), kv4_offset(pr)), o[i]);
+        const int d = lane * kMine + i, k = d % 8 / 2;
+        const int step = d / 32 * 2 + k / 2;
+        const __half v = __float2half_rn(x[i] * up * (k & 1 ? 0.0625f : 1.0f));
+        reinterpret_cast<__half *>(qs)[((((r / 8) * (D / 16) + step) * 32 + (r % 8) * 4 + d % 32 / 8) * 2 + (k & 1)) * 2 +
+                                       (d & 1)] = v;
+      }
+      const float s2 = a.scale * kLog2e;
+      if (lane == 0) {
+        q_scale[r] = __uint_as_float((uint32_t)(24 - 14 + e + 127) << 23) * s2;
+        limits[r] = row_limit(a, it, min(row, it.qn * a.ratio - 1));
+      }
+      if (lane % (32 / NG) == 0) q_sum[lane / (32 / NG) * F::kRows + r] = sum * s2;
+    }
+    __syncthreads();
+    uint32_t qf[F::kQRegs ? D / 16 : 1][2];
+    if constexpr (F::kQRegs) {
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        const uint2 v = reinterpret_cast<const uint2 *>(qs)[i * 32 + lane];
+        qf[i][0] = v.x, qf[i][1] = v.y;
       }
     }
-  }
-  for (int x = 16; x; x >>= 1) l += __shfl_xor_sync(0xffffffffu, l, x);
-  T *out = static_cast<T *>(a.out) + ((int64_t)row * a.q_heads + head) * D;
+    const int sees_least = limits[0], sees_most = limits[F::kRows - 1];
+
+    float o[D / 16][NT][4], z[NT][2][NG], l[NT][2], over[NT][2], sub[NT][2];
 #pragma unroll
-  for (int i = 0; i < kMine; ++i) out[i * 32 + lane] = kv4_round<T>(l > 0.0f ? o[i] / l : (l == 0.0f ? 0.0f : l));
-  if (a.lse && lane == 0)
-    a.lse[(int64_t)row * a.q_heads + head] = l == 0.0f ? -INFINITY : m * 0.6931471805599453f + logf(l);
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[i][n][e] = 0.0f;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        l[n][h] = 0.0f;
+        over[n][h] = -INFINITY;  // the running maximum plus kSlack
+        sub[n][h] = 0.0f;        // the running maximum, 0 before there is one
+#pragma unroll
+        for (int gi = 0; gi < NG; ++gi) z[n][h][gi] = 0.0f;
+      }
+    }
+    auto recentre = [&]() {  // o += z, summed over the lanes that share a row
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int gi = 0; gi < NG; ++gi) {
+            float x = z[n][h][gi];
+            x += __shfl_xor_sync(0xffffffffu, x, 4);
+            x += __shfl_xor_sync(0xffffffffu, x, 8);
+            x += __shfl_xor_sync(0xffffffffu, x, 16);
+            z[n][h][gi] = 0.0f;
+#pragma unroll
+            for (int i = gi * F::kGroupWords * 2; i < (gi + 1) * F::kGroupWords * 2; ++i) {
+              o[i][n][h] = fmaf(x, 0x1p-24f, o[i][n][h]);
+              o[i][n][2 + h] = fmaf(x, 0x1p-20f, o[i][n][2 + h]);
+            }
+          }
+    };
+
+    int since = 0;
+#pragma unroll 1
+    for (; unit < end; unit += kWarps) {
+      const int tile = (int)(unit - first);
+      if (held >> stage & 1) {
+        const uint8_t *buf = ring + stage * F::kTile;
+        if (!bar_wait(bars + 8 * stage, parity >> stage & 1)) kv4_error(c.errors, kErrTimeout);
+        parity ^= 1u << stage;
+        // ---- scores
+        float s[NT][4];
+        uint32_t par[2][NG];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) load_words<NG>(buf + 16 * D + (g + 8 * h) * NG * 4, par[h]);
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s[n][e] = 0.0f;
+        uint32_t w0[F::kWpr], w1[F::kWpr];
+        float acc[NT][4];
+#pragma unroll
+        for (int i = 0; i < F::kWords; ++i) {
+          if (i % F::kWpr == 0) {
+            const uint8_t *p = buf + (i / F::kWpr) * 16 * 16 * F::kWpr + g * 16 * F::kWpr + t * 4 * F::kWpr;
+            load_words<F::kWpr>(p, w0);
+            load_words<F::kWpr>(p + 8 * 16 * F::kWpr, w1);
+          }
+          if (i % F::kGroupWords == 0) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) acc[n][e] = 0.0f;
+          }
+          uint32_t x = w0[i % F::kWpr], y = w1[i % F::kWpr];
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t a0 = x & 0x000f000fu, a1 = y & 0x000f000fu, a2 = x & 0x00f000f0u, a3 = y & 0x00f000f0u;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              if constexpr (F::kQRegs) {
+                mma(acc[n], a0, a1, a2, a3, qf[2 * i + half][0], qf[2 * i + half][1]);
+              } else {
+                const uint2 b = reinterpret_cast<const uint2 *>(qs)[(n * (D / 16) + 2 * i + half) * 32 + lane];
+                mma(acc[n], a0, a1, a2, a3, b.x, b.y);
+              }
+            }
+            x >>= 8, y >>= 8;
+          }
+          if (i % F::kGroupWords == F::kGroupWords - 1) {
+            const int gi = i / F::kGroupWords;
+            const float s0 = kv4_scale(par[0][gi]), s1 = kv4_scale(par[1][gi]);
+            const float b0 = fmaf(-8.0f, s0, kv4_offset(par[0][gi])), b1 = fmaf(-8.0f, s1, kv4_offset(par[1][gi]));
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              const float2 qa = *reinterpret_cast<const float2 *>(q_scale + n * 8 + 2 * t);
+              const float2 qb = *reinterpret_cast<const float2 *>(q_sum + gi * F::kRows + n * 8 + 2 * t);
+              s[n][0] += fmaf(s0, acc[n][0] * qa.x, b0 * qb.x);
+              s[n][1] += fmaf(s0, acc[n][1] * qa.y, b0 * qb.y);
+              s[n][2] += fmaf(s1, acc[n][2] * qa.x, b1 * qb.x);
+              s[n][3] += fmaf(s1, acc[n][3] * qa.y, b1 * qb.y);
+            }
+          }
+        }
+        // ---- V: everything leaves the ring here, so that the next tile may come in
+        uint32_t vpar[2][NG], vw[2][F::kWords];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          load_words<NG>(buf + 16 * D + 64 * NG + (g + 8 * h) * NG * 4, vpar[h]);
+#pragma unroll
+          for (int sl = 0; sl < F::kSlabs; ++sl)
+            load_words<F::kWpr>(buf + 8 * D + ((sl * 2 + h) * 32 + lane) * 4 * F::kWpr, vw[h] + sl * F::kWpr);
+        }
+        __syncwarp();
+        ahead_issue(stage);
+
+        // ---- weights. Rows of tokens t0 + g and t0 + g + 8.
+        const int tok = tile * kKv4Tile + g;
+        const bool partial = (tile + 1) * kKv4Tile > sees_least;
+        if (partial) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            const int2 lim = *reinterpret_cast<const int2 *>(limits + n * 8 + 2 * t);
+            s[n][0] = tok < lim.x ? s[n][0] : -INFINITY;
+            s[n][1] = tok < lim.y ? s[n][1] : -INFINITY;
+            s[n][2] = tok + 8 < lim.x ? s[n][2] : -INFINITY;
+            s[n][3] = tok + 8 < lim.y ? s[n][3] : -INFINITY;
+          }
+#pragma unroll
+          for (int gi = 0; gi < NG; ++gi) {
+            if (tok >= sees_most) vpar[0][gi] = 0;
+            if (tok + 8 >= sees_most) vpar[1][gi] = 0;
+          }
+        }
+        // p' = p * scale_v stays near 1 if the maximum is taken over s + log2 scale_v
+        float ev[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float top = 0x1p-24f;
+#pragma unroll
+          for (int gi = 0; gi < NG; ++gi) top = fmaxf(top, kv4_scale(vpar[h][gi]));
+          ev[h] = (float)((int)(__float_as_uint(top) >> 23) - 127);
+        }
+        bool raise = false;
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) raise |= s[n][e] + ev[e >> 1] > over[n][e & 1];
+        if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              float m = fmaxf(s[n][h] + ev[0], s[n][2 + h] + ev[1]);
+              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
+              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
+              m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
+              const bool fresh = over[n][h] == -INFINITY;
+              if (m == -INFINITY || (!fresh && m <= sub[n][h])) continue;
+              const float f = fresh ? 1.0f : ex2(sub[n][h] - m);
+              sub[n][h] = m;
+              over[n][h] = m + kSlack;
+              l[n][h] *= f;
+#pragma unroll
+              for (int gi = 0; gi < NG; ++gi) z[n][h][gi] *= f;
+#pragma unroll
+              for (int i = 0; i < D / 16; ++i) {
+                o[i][n][h] *= f;
+                o[i][n][2 + h] *= f;
+              }
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            s[n][e] = ex2(s[n][e] - sub[n][e & 1]);
+            l[n][e & 1] += s[n][e];
+          }
+        // ---- O += V P'
+#pragma unroll
+        for (int gi = 0; gi < NG; ++gi) {
+          const float s0 = kv4_scale(vpar[0][gi]), s1 = kv4_scale(vpar[1][gi]);
+          const float f0_ = kv4_offset(vpar[0][gi]), f1_ = kv4_offset(vpar[1][gi]);
+          uint32_t b[NT][2];
+#pragma unroll
+          for (int n = 0; n < NT; ++n) {
+            float p0 = s[n][0] * s0, p1 = s[n][1] * s0, p2 = s[n][2] * s1, p3 = s[n][3] * s1;
+            float y0 = s[n][0] * f0_, y1 = s[n][1] * f0_, y2 = s[n][2] * f1_, y3 = s[n][3] * f1_;
+            if (partial) {  // a weight of 0 beside an infinite or NaN scale is nothing
+              if (s[n][0] == 0.0f) p0 = y0 = 0.0f;
+              if (s[n][1] == 0.0f) p1 = y1 = 0.0f;
+              if (s[n][2] == 0.0f) p2 = y2 = 0.0f;
+              if (s[n][3] == 0.0f) p3 = y3 = 0.0f;
+            }
+            const __half2 h0 = __floats2half2_rn(p0, p1), h1 = __floats2half2_rn(p2, p3);
+            const float2 r0 = __half22float2(h0), r1 = __half22float2(h1);
+            z[n][0][gi] += (y0 + y2) - 8.0f * (r0.x + r1.x);
+            z[n][1][gi] += (y1 + y3) - 8.0f * (r0.y + r1.y);
+            b[n][0] = transpose8(*reinterpret_cast<const uint32_t *>(&h0));
+            b[n][1] = transpose8(*reinterpret_cast<const uint32_t *>(&h1));
+          }
+#pragma unroll
+          for (int i = gi * F::kGroupWords; i < (gi + 1) * F::kGroupWords; ++i) {
+            uint32_t x = vw[0][i], y = vw[1][i];
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+              const uint32_t a0 = x & 0x000f000fu, a1 = x & 0x00f000f0u, a2 = y & 0x000f000fu, a3 = y & 0x00f000f0u;
+#pragma unroll
+              for (int n = 0; n < NT; ++n) mma(o[2 * i + half][n], a0, a1, a2, a3, b[n][0], b[n][1]);
+              x >>= 8, y >>= 8;
+            }
+          }
+        }
+        // Codes are sums around 7.5 scale until they are centred; the tensor
+        // cores cut low bits off a sum, which would add up over a long row.
+        if (++since == kRecentre) {
+          recentre();
+          since = 0;
+        }
+      } else {
+        ahead_issue(stage);
+      }
+      stage = stage + 1 == F::kStages ? 0 : stage + 1;
+    }
+    recentre();
+
+    // ---- the eight warps' results, one n-tile at a time
+    const bool whole = seg == first && end == first + it.tiles;
+    float *part = a.parts + ((long long)blockIdx.x * 2 + (first_segment ? 0 : 1)) * F::kPart;
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      if (n) __syncthreads();
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float sum = l[n][h];
+        sum += __shfl_xor_sync(0xffffffffu, sum, 4);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 8);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 16);
+        float *to = merge + (warp * 8 + 2 * t + h) * F::kOutStride + g;
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+          to[16 * i] = o[i][n][h] * 0x1p24f;
+          to[16 * i + 8] = o[i][n][2 + h] * 0x1p20f;
+        }
+        if (g == 0) {
+          merge_ml[(warp * 8 + 2 * t + h) * 2] = over[n][h] == -INFINITY && sum == 0.0f ? -INFINITY : sub[n][h];
+          merge_ml[(warp * 8 + 2 * t + h) * 2 + 1] = sum;
+        }
+      }
+      __syncthreads();
+      const int r = n * 8 + warp;
+      if (r < rows) {
+        float m = -INFINITY, sum = 0.0f, f[kWarps];
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) m = fmaxf(m, merge_ml[(w * 8 + warp) * 2]);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) {
+          const float mw = merge_ml[(w * 8 + warp) * 2];
+          f[w] = mw == -INFINITY ? 0.0f : ex2(mw - m);
+          sum += mw == -INFINITY ? 0.0f : f[w] * merge_ml[(w * 8 + warp) * 2 + 1];
+        }
+        const int row = it.rt * F::kRows + r;
+        const int64_t at = (int64_t)(it.q0 + row / a.ratio) * a.q_heads + it.h * a.ratio + row % a.ratio;
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+        for (int i = 0; i < D / 64; ++i) {
+          const int d = i * 64 + lane * 2;
+          float x = 0.0f, y = 0.0f;
+#pragma unroll
+          for (int w = 0; w < kWarps; ++w) {
+            const float2 v = *reinterpret_cast<const float2 *>(merge + (w * 8 + warp) * F::kOutStride + d);
+            if (f[w] != 0.0f) x = fmaf(f[w], v.x, x), y = fmaf(f[w], v.y, y);
+          }
+          if (!whole) {
+            *reinterpret_cast<float2 *>(part + r * D + d) = make_float2(x, y);
+          } else if (a.bf16) {
+            reinterpret_cast<__nv_bfloat162 *>(a.out)[(at * D + d) / 2] = __floats2bfloat162_rn(x * inv, y * inv);
+          } else {
+            reinterpret_cast<__half2 *>(a.out)[(at * D + d) / 2] = __floats2half2_rn(x * inv, y * inv);
+          }
+        }
+        if (lane == 0) {
+          if (!whole) {
+            part[F::kRows * D + 2 * r] = m;
+            part[F::kRows * D + 2 * r + 1] = sum;
+          } else if (a.lse) {
+            a.lse[at] = sum == 0.0f ? -INFINITY : (m + log2f(sum)) * kLn2;
+          }
+        }
+      }
+    }
+    if (seg == first && end < first + it.tiles) {  // begun here, ended elsewhere
+      const long long last = (first + it.tiles - 1) / share;
+      join = make_int4(it.b, it.rt, it.h, (int)(last - blockIdx.x + 1) * 2 + (first_segment ? 0 : 1));
+    }
+    first_segment = false;
+    seg = end;
+    if (seg < f1) {
+      first += it.tiles;
+      next_item<F::kRows>(a, c.kv_heads, most, it);
+    }
+  }
+  if (threadIdx.x == 0) a.joins[blockIdx.x] = join;
 }
+
+// Joins the parts of the items that CTAs of the first kernel began and did not
+// end: block (x, r) does row r of CTA x's. Parts are taken in order.
+template <int D>
+__global__ void __launch_bounds__(D) attend_join_kernel(const Kv4View c, const AttendArgs a, const int tile_rows) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int4 join = a.joins[blockIdx.x];
+  const int n = join.w >> 1;
+  if (n == 0) return;
+  Item it;
+  it.b = join.x, it.rt = join.y, it.h = join.z;
+  load_request(a, (int)min((long long)a.columns * c.page_size, 0x7fffffffll), it.b, it.q0, it.qn, it.len);
+  const int r = blockIdx.y, row = it.rt * tile_rows + r;
+  if (row >= it.qn * a.ratio) return;
+  const int size = tile_rows * (D + 2);
+  const float *one = a.parts + ((long long)blockIdx.x * 2 + (join.w & 1)) * size;
+  const float *rest = a.parts + ((long long)blockIdx.x * 2) * size;
+  float m = -INFINITY, sum = 0.0f, x = 0.0f;
+#pragma unroll 4
+  for (int i = 0; i < n; ++i) m = fmaxf(m, (i ? rest + (long long)i * 2 * size : one)[tile_rows * D + 2 * r]);
+#pragma unroll 4
+  for (int i = 0; i < n; ++i) {
+    const float *p = i ? rest + (long long)i * 2 * size : one;
+    const float mi = p[tile_rows * D + 2 * r], li = p[tile_rows * D + 2 * r + 1], v = p[r * D + threadIdx.x];
+    if (mi == -INFINITY) continue;
+    const float f = ex2(mi - m);
+    if (f != 0.0f) x = fmaf(f, v, x), sum = fmaf(f, li, sum);
+  }
+  const int64_t at = (int64_t)(it.q0 + row / a.ratio) * a.q_heads + it.h * a.ratio + row % a.ratio;
+  x = sum == 0.0f ? 0.0f : x / sum;
+  if (a.bf16) static_cast<__nv_bfloat16 *>(a.out)[at * D + threadIdx.x] = __float2bfloat16_rn(x);
+  else static_cast<__half *>(a.out)[at * D + threadIdx.x] = __float2half_rn(x);
+  if (a.lse && threadIdx.x == 0) a.lse[at] = sum == 0.0f ? -INFINITY : (m + log2f(sum)) * kLn2;
+}
+
+// ------------------------------------------------------------------- the host
+
+struct Launch {
+  int rows;      // of a row tile
+  int ctas;
+  int part;      // floats of a partial result
+};
+
+constexpr int kMaxDevices = 64;
+
+int sm_count(int device) {
+  static int known[kMaxDevices] = {};
+  if (device < 0 || device >= kMaxDevices) return 148;
+  if (!known[device]) {
+    int n = 0;
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || n <= 0) n = 148;
+    known[device] = n;
+  }
+  return known[device];
+}
+
+template <int D, int NG, int NT>
+cudaError_t run_few(const Kv4View &c, const AttendArgs &a, const Launch &l, cudaStream_t stream) {
+  using F = Form<D, NG, NT>;
+  cudaError_t e =
+      cudaFuncSetAttribute(attend_few_kernel<D, NG, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem);
+  if (e != cudaSuccess) return e;
+  attend_few_kernel<D, NG, NT><<<l.ctas, kThreads, F::kSmem, stream>>>(c, a);
+  if ((e = cudaGetLastError()) != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(l.ctas, F::kRows);
+  cfg.blockDim = dim3(D);
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, attend_join_kernel<D>, c, a, (int)F::kRows);
+}
+
+// f(integral constants D, NG, NT) for a cache and a number of n-tiles.
+template <typename F>
+auto by_form(int d, int ng, int nt, F f) {
+  auto with_nt = [&](auto dd, auto gg) {
+    constexpr int kD = decltype(dd)::value;
+    if (nt == 1) return f(dd, gg, std::integral_constant<int, 1>{});
+    if (nt == 2 || kD > 128) return f(dd, gg, std::integral_constant<int, 2>{});
+    return f(dd, gg, std::integral_constant<int, (kD > 128 ? 2 : 4)>{});
+  };
+  auto with_ng = [&](auto dd) {
+    constexpr int kD = decltype(dd)::value;
+    if (ng == 1) return with_nt(dd, std::integral_constant<int, 1>{});
+    if (ng == 2 || kD < 128) return with_nt(dd, std::integral_constant<int, 2>{});
+    if (ng == 4 || kD < 256) return with_nt(dd, std::integral_constant<int, (kD < 128 ? 2 : 4)>{});
+    return with_nt(dd, std::integral_constant<int, (kD < 256 ? kD / 32 : 8)>{});
+  };
+  if (d == 64) return with_ng(std::integral_constant<int, 64>{});
+  if (d == 128) return with_ng(std::integral_constant<int, 128>{});
+  return with_ng(std::integral_constant<int, 256>{});
+}
+
+// Row tiles of 8, 16 or 32 rows: the smallest that holds the rows of a
+// request, so that the cache is read once. Larger ones would leave no
+// registers (O is D*rows/32 of them in a lane), so more rows are more tiles.
+int few_tiles(int head_dim, int64_t rows) {
+  if (rows <= 8) return 1;
+  return rows <= 16 || head_dim > 128 ? 2 : 4;
+}
+
+Launch plan_launch(const cb_kv4_cache *cache, const cb_kv4_attend_args *a) {
+  const int64_t ratio = a->q_heads / cache->kv_heads;
+  const int nt = few_tiles(cache->head_dim, ratio * (a->max_q > 1 ? a->max_q : 1));
+  Launch l;
+  l.rows = 8 * nt;
+  l.part = l.rows * (cache->head_dim + 2);
+  l.ctas = sm_count(cache->device) * (nt == 1 && cache->head_dim <= 128 ? 2 : 1);
+  return l;
+}
+
+uint64_t workspace_bytes(const Launch &l) { return (uint64_t)l.ctas * (16 + 8ull * l.part); }
 
 int check(const cb_kv4_cache *cache, const cb_kv4_attend_args *a, Kv4View *c) {
   if (!a) return kv4_fail(CB_ERR_ARG, "cb_kv4_attend: no arguments");
@@ -140,9 +839,10 @@ int check(const cb_kv4_cache *cache, const cb_kv4_attend_args *a, Kv4View *c) {
 }  // namespace cb
 
 extern "C" uint64_t cb_kv4_attend_workspace(const cb_kv4_cache *cache, const cb_kv4_attend_args *a) {
-  (void)cache;
-  (void)a;
-  return 0;
+  using namespace cb;
+  Kv4View c;
+  if (check(cache, a, &c) != CB_OK) return 0;
+  return workspace_bytes(plan_launch(cache, a));
 }
 
 extern "C" int cb_kv4_attend(const cb_kv4_cache *cache, const cb_kv4_attend_args *args, void *stream) {
@@ -150,6 +850,10 @@ extern "C" int cb_kv4_attend(const cb_kv4_cache *cache, const cb_kv4_attend_args
   Kv4View c;
   if (int rc = check(cache, args, &c)) return rc;
   if (args->requests == 0 || args->total_q == 0) return CB_OK;
+  const Launch l = plan_launch(cache, args);
+  if (!args->workspace || args->workspace_bytes < workspace_bytes(l) ||
+      (reinterpret_cast<uintptr_t>(args->workspace) & 15))
+    return kv4_fail(CB_ERR_ARG, "cb_kv4_attend: workspace too small or not 16-byte aligned");
   Kv4Device dev(cache->device);
   if (dev.err != cudaSuccess) return kv4_fail(CB_ERR_CUDA, "cb_kv4_attend: device", dev.err);
   AttendArgs a = {};
@@ -162,28 +866,21 @@ extern "C" int cb_kv4_attend(const cb_kv4_cache *cache, const cb_kv4_attend_args
   a.table_stride = args->table_stride;
   a.q_token_stride = args->q_token_stride;
   a.q_head_stride = args->q_head_stride;
+  a.joins = static_cast<int4 *>(args->workspace);
+  a.parts = reinterpret_cast<float *>(a.joins + l.ctas);
   a.scale = args->scale;
   a.requests = args->requests;
   a.columns = args->columns;
   a.total_q = args->total_q;
   a.q_heads = args->q_heads;
+  a.ratio = args->q_heads / cache->kv_heads;
   a.causal = args->causal;
-  a.group = cache->group;
-  const int64_t warps = (int64_t)a.total_q * a.q_heads;
-  if ((warps + 3) / 4 > 0x7fffffff) return kv4_fail(CB_ERR_ARG, "cb_kv4_attend: too many rows");
-  const unsigned grid = (unsigned)((warps + 3) / 4);
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const bool half = args->dtype == CB_KV4_F16;
-  if (cache->head_dim == 64) {
-    if (half) attend_kernel<__half, 64><<<grid, 128, 0, st>>>(c, a);
-    else attend_kernel<__nv_bfloat16, 64><<<grid, 128, 0, st>>>(c, a);
-  } else if (cache->head_dim == 128) {
-    if (half) attend_kernel<__half, 128><<<grid, 128, 0, st>>>(c, a);
-    else attend_kernel<__nv_bfloat16, 128><<<grid, 128, 0, st>>>(c, a);
-  } else {
-    if (half) attend_kernel<__half, 256><<<grid, 128, 0, st>>>(c, a);
-    else attend_kernel<__nv_bfloat16, 256><<<grid, 128, 0, st>>>(c, a);
-  }
-  const cudaError_t e = cudaGetLastError();
+  a.bf16 = args->dtype == CB_KV4_BF16;
+  a.min_share = kWarps;
+  const cudaError_t e = by_form(cache->head_dim, cache->head_dim / cache->group, l.rows / 8,
+                                [&](auto d, auto ng, auto nt) {
+                                  return run_few<decltype(d)::value, decltype(ng)::value, decltype(nt)::value>(
+                                      c, a, l, static_cast<cudaStream_t>(stream));
+                                });
   return e == cudaSuccess ? CB_OK : kv4_fail(CB_ERR_CUDA, "cb_kv4_attend: launch", e);
 }
