@@ -446,7 +446,7 @@ uint64_t cb_kv4_page_bytes(int32_t layers, int32_t kv_heads, int32_t head_dim, i
  * page_size + offset) and positions (kv_len + j). Missing pages come off the
  * end of the stack, rows in order. A row is refused (status CB_PUT_FAILED, its
  * slots -1, its length kept) if its tokens end past `tokens`, if they pass
- * columns * page_size, or if it needs pages and the rows up to it need more
+ * columns * page_size (at most 2^30), or if it needs pages and the rows up to it need more
  * than the stack has; a refused row's pages still count for the rows behind
  * it. Entries behind the last token get slot -1, position 0. kv_lens_out
  * and free_count_out may be kv_lens and free_count. */
@@ -487,8 +487,9 @@ int cb_kv4_read(const cb_kv4_cache *cache, int32_t layer, int32_t dtype, void *k
  * [total_q][q_heads][head_dim] and the tokens 0 .. kv_lens[i] of its pages
  * block_table[i][..]; row r of its n rows sees the tokens below kv_len - (n -
  * 1 - r) when causal, else all of them. q_heads is a multiple of kv_heads. A
- * row that sees nothing gets zeros and lse -inf. out: [total_q][q_heads]
- * [head_dim] dense, of q's type; lse (natural log, [total_q][q_heads] fp32) or
+ * row that sees nothing gets zeros and lse -inf; columns * page_size is at most
+ * 2^30. out: [total_q][q_heads]
+ * [head_dim] dense, 16-byte aligned, of q's type; lse (natural log, [total_q][q_heads] fp32) or
  * NULL. Rows behind q_start[requests] are left as they were. max_q is a hint
  * (rows of a request at most); results do not depend on it being right.
  * workspace: cb_kv4_attend_workspace bytes, 16-byte aligned, used until the

@@ -222,8 +222,8 @@ class KV4Cache(KVPageConnector):
         if out is None:
             out = torch.empty((rows, heads, d), dtype=q.dtype, device=dev)
         elif (not isinstance(out, torch.Tensor) or out.device != dev or out.dtype != q.dtype
-              or out.shape != q.shape or not out.is_contiguous()):
-            raise ValueError("out must be contiguous and like q")
+              or out.shape != q.shape or not out.is_contiguous() or out.data_ptr() % 16):
+            raise ValueError("out must be contiguous, 16-byte aligned and like q")
         elif rows and out.data_ptr() == q.data_ptr():
             raise ValueError("out may not be q")
         lse = torch.empty((rows, heads), dtype=torch.float32, device=dev) if return_lse else None
@@ -270,8 +270,8 @@ class PageTable:
     def __init__(self, requests: int, columns: int, num_pages: int, page_size: int = 16, device=None):
         if requests < 0 or columns <= 0 or num_pages <= 0 or page_size <= 0:
             raise ValueError("requests, columns, num_pages and page_size must be positive")
-        if columns * page_size > 0x7fffffff:
-            raise ValueError("a row may not hold more than 2^31 - 1 tokens")
+        if columns * page_size > 1 << 30:
+            raise ValueError("a row may not hold more than 2^30 tokens")
         self.device = _device(device)
         self.requests, self.columns, self.num_pages = int(requests), int(columns), int(num_pages)
         self.page_size = int(page_size)

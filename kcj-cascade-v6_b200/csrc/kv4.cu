@@ -464,8 +464,8 @@ extern "C" int cb_kv4_plan(const cb_kv4_plan_args *a, void *stream) {
   if (!a || a->requests < 0 || a->tokens < 0 || a->columns <= 0 || a->num_pages <= 0 || a->page_size <= 0 ||
       a->table_stride < a->columns)
     return kv4_fail(CB_ERR_ARG, "cb_kv4_plan: bad sizes");
-  if ((long long)a->columns * a->page_size > 0x7fffffffll)
-    return kv4_fail(CB_ERR_ARG, "cb_kv4_plan: a row may not hold more than 2^31 - 1 tokens");
+  if ((long long)a->columns * a->page_size > kKv4MostTokens)
+    return kv4_fail(CB_ERR_ARG, "cb_kv4_plan: a row may not hold more than 2^30 tokens");
   if (!a->free || !a->free_count || !a->free_count_out || !a->q_start || (a->tokens > 0 && (!a->slots || !a->positions)) ||
       (a->requests > 0 && (!a->q_lens || !a->kv_lens || !a->kv_lens_out || !a->block_table || !a->status)) ||
       (a->done && !a->borrowed))

@@ -29,6 +29,7 @@ namespace cb {
 
 constexpr int kKv4Tile = 16;             // tokens of a tile
 constexpr float kKv4Most = 65000.0f;     // larger values are stored as this one
+constexpr long long kKv4MostTokens = 1 << 30;  // of a row of a block table: positions stay clear of 2^31
 
 CB_HD int kv4_slab(int d) { return d < 128 ? d : 128; }
 CB_HD int kv4_tile_bytes(int d, int group) { return 16 * d + 128 * (d / group); }

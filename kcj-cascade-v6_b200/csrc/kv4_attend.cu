@@ -35,7 +35,10 @@ namespace {
 // by a power of two per row: exact for fp16 and, above 2^-28 of the row's
 // largest, for bf16.
 constexpr int kWarps = 8, kThreads = kWarps * 32;
-constexpr int kRecentre = 8;      // tiles between centrings of the sums
+constexpr int kRecentre = 4;      // pairs of tiles between centrings of the sums
+// What an item costs a CTA beside its tiles (query rows in, eight warps'
+// results joined), in tiles: it takes this much of the line too.
+constexpr int kItemCost = 12;
 constexpr float kSlack = 8.0f;    // p may reach 2^8 before the maximum is raised
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr uint32_t kWaitLimit = 1u << 24;
@@ -67,17 +70,20 @@ struct Form {
   static constexpr int kWpr = D / kSlabs / 32;      // words a lane reads of a row and slab
   static constexpr int kWords = D / 32;
   static constexpr int kGroupWords = kWords / NG;
-  // bytes in flight: 8 or 16 warps with 4 tiles of 1.2 - 2.6 KB are 70 KB and more on
-  // an SM; HBM needs about 6.5 TB/s * 0.8 us / 148 = 35 KB
-  static constexpr int kStages = D > 128 || NG > 2 ? 3 : 4;
+  // A warp's ring is two pairs of tiles. Bytes in flight: 8 or 16 warps with 2 to 4
+  // tiles of 1.2 - 5.1 KB are 35 KB and more on an SM; HBM needs about
+  // 6.5 TB/s * 0.8 us / 148 = 35 KB.
+  static constexpr int kJoint = NT == 1 ? 2 : 1;  // tiles whose products run side by side
   static constexpr int kCtasPerSm = NT == 1 && D <= 128 ? 2 : 1;
-  static constexpr bool kQRegs = NT == 1 && D <= 128;
-  static constexpr int kOutStride = D + 4;          // two rows are 8 banks apart
-  static constexpr int kRing = kWarps * kStages * kTile;
+  static constexpr bool kQRegs = NT == 1 && D <= 128 && NG == 1;
+  static constexpr bool kOnes = NT * NG <= 2;
+  static constexpr int kMergeD = D / kSlabs;        // dims joined at once
+  static constexpr int kOutStride = kMergeD + 4;    // two rows are 8 banks apart
+  static constexpr int kRing = kWarps * 4 * kTile;
   static constexpr int kQ = NT * (D / 16) * 32 * 8;
   static constexpr int kConst = kRows * (2 + NG) * 4;
   static constexpr int kMerge = kWarps * 8 * (kOutStride + 2) * 4;
-  static constexpr int kSmem = kRing + kQ + kMerge + kConst + kWarps * kStages * 8 + 128;
+  static constexpr int kSmem = kRing + kQ + kMerge + kConst + kWarps * 16;
   static constexpr int kPart = kRows * (D + 2);     // floats of a partial result
 };
 
@@ -110,6 +116,15 @@ CB_D void mma(float *c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// u0, u1 += the sum over 16 rows of the columns 2t, 2t + 1 of b.
+CB_D void mma_sum(float &u0, float &u1, uint32_t b0, uint32_t b1) {
+  [[maybe_unused]] float x, y;  // rows 8..15 of the product
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%6,%7,%6,%7}, {%4,%5}, {%0,%1,%8,%8};"
+      : "+f"(u0), "+f"(u1), "=f"(x), "=f"(y)
+      : "r"(b0), "r"(b1), "r"(0x3c003c00u), "r"(0u), "f"(0.0f));
 }
 
 CB_D uint32_t transpose8(uint32_t x) {
@@ -163,7 +178,7 @@ CB_D void item_tiles(const AttendArgs &a, Item &it) {
   it.tiles = max(1, (row_limit(a, it, last) + kKv4Tile - 1) / kKv4Tile);
 }
 
-// Tiles of all items of request b.
+// What all items of request b take of the line.
 template <int ROWS>
 CB_D long long request_tiles(const AttendArgs &a, int heads, int most, int b) {
   Item it;
@@ -172,7 +187,7 @@ CB_D long long request_tiles(const AttendArgs &a, int heads, int most, int b) {
   const int rts = (it.qn * a.ratio + ROWS - 1) / ROWS;
   for (it.rt = 0; it.rt < rts; ++it.rt) {
     item_tiles<ROWS>(a, it);
-    n += it.tiles;
+    n += it.tiles + kItemCost;
   }
   return n * heads;
 }
@@ -198,8 +213,8 @@ CB_D long long warp_sum(long long x) {
   return x;
 }
 
-// Finds this CTA's piece [f0, f1) of the line of units and the item that holds
-// f0 (its first unit is `first`). All threads return the same.
+// Finds this CTA's piece [f0, f1) of the line and the item that holds f0, which
+// begins at `first`. All threads return the same.
 template <int ROWS>
 CB_D bool find_piece(const AttendArgs &a, const Kv4View &c, int most, long long &share, long long &f0, long long &f1,
                      long long &first, Item &it) {
@@ -257,12 +272,35 @@ CB_D bool find_piece(const AttendArgs &a, const Kv4View &c, int most, long long 
   load_request(a, most, it.b, it.q0, it.qn, it.len);
   for (it.rt = 0;; ++it.rt) {
     item_tiles<ROWS>(a, it);
-    const long long n = (long long)it.tiles * c.kv_heads;
+    const long long n = (long long)(it.tiles + kItemCost) * c.kv_heads;
     if (f0 < first + n) break;
     first += n;
   }
-  it.h = (int)((f0 - first) / it.tiles);
-  first += (long long)it.h * it.tiles;
+  it.h = (int)((f0 - first) / (it.tiles + kItemCost));
+  first += (long long)it.h * (it.tiles + kItemCost);
+  return true;
+}
+
+// A CTA's piece of the line, item by item: the item and its tiles [t0, t1) in
+// the piece. Positions count from the piece's beginning.
+struct Walk {
+  Item it;
+  int at;  // of the item's first tile; not positive if it began in an earlier CTA
+  int t0, t1;
+  CB_D void cut(int units) {
+    t0 = max(0, -at);
+    t1 = min(it.tiles, units - at);
+  }
+};
+
+// The next item of the piece that has tiles in it; false behind the last.
+template <int ROWS>
+CB_D bool next_in_piece(const AttendArgs &a, int heads, int most, int units, Walk &w) {
+  do {
+    w.at += w.it.tiles + kItemCost;
+    if (w.at >= units || !next_item<ROWS>(a, heads, most, w.it)) return false;
+    w.cut(units);
+  } while (w.t1 <= w.t0);
   return true;
 }
 
@@ -270,8 +308,7 @@ template <int D, int NG, int NT>
 __global__ void __launch_bounds__(kThreads, Form<D, NG, NT>::kCtasPerSm)
     attend_few_kernel(const Kv4View c, const AttendArgs a) {
   using F = Form<D, NG, NT>;
-  extern __shared__ uint8_t raw[];
-  uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 127) & ~(uintptr_t)127);
+  extern __shared__ __align__(128) uint8_t smem[];
   uint32_t *qs = reinterpret_cast<uint32_t *>(smem + F::kRing);
   float *merge = reinterpret_cast<float *>(smem + F::kRing + F::kQ);
   float *merge_ml = merge + kWarps * 8 * F::kOutStride;
@@ -279,74 +316,87 @@ __global__ void __launch_bounds__(kThreads, Form<D, NG, NT>::kCtasPerSm)
   int *limits = reinterpret_cast<int *>(q_scale + F::kRows);
   float *q_sum = reinterpret_cast<float *>(limits + F::kRows);  // [NG][rows]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  uint8_t *ring = smem + warp * F::kStages * F::kTile;
-  const uint32_t bars =
-      smem_addr(smem + F::kRing + F::kQ + F::kMerge + F::kConst) + (uint32_t)warp * F::kStages * 8;
-  const int most = (int)min((long long)a.columns * c.page_size, 0x7fffffffll);
+  const uint8_t *ring = smem + warp * 4 * F::kTile;
+  const uint32_t ring_at = smem_addr(ring);
+  const uint32_t bars = smem_addr(smem + F::kRing + F::kQ + F::kMerge + F::kConst) + warp * 16;
+  const int most = a.columns * c.page_size;
   const int per_page = c.page_log2 - 4;
 
   asm volatile("griddepcontrol.launch_dependents;");
   if (lane == 0) {
-    for (int i = 0; i < F::kStages; ++i) bar_init(bars + 8 * i, 1);
+    bar_init(bars, 2);  // two lanes arrive, one for each tile
+    bar_init(bars + 8, 2);
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   __syncwarp();
   long long share, f0, f1, first;
-  Item it;
-  if (!find_piece<F::kRows>(a, c, most, share, f0, f1, first, it)) {
+  Walk w;
+  if (!find_piece<F::kRows>(a, c, most, share, f0, f1, first, w.it)) {
     if (threadIdx.x == 0) a.joins[blockIdx.x] = make_int4(0, 0, 0, 0);
     return;
   }
+  const int units = (int)(f1 - f0);
+  w.at = (int)(first - f0) + kItemCost;
+  w.cut(units);
+  bool more = w.t1 > w.t0 || next_in_piece<F::kRows>(a, c.kv_heads, most, units, w);
 
-  // The warp's units are f0 + warp + 8 i. `ahead` runs kStages of them before
-  // the products, with the page of its next unit already asked for.
-  Item ahead = it;
-  long long a_unit = f0 + warp, a_first = first;
-  int a_page = -1;
-  bool a_there = a_unit < f1;
-  uint32_t held = 0, parity = 0;  // a bit for each stage: has data; wait parity
-  auto ahead_find = [&]() {  // moves to the item of a_unit and asks for its page
-    a_there = a_unit < f1;
-    while (a_there && a_unit >= a_first + ahead.tiles) {
-      a_first += ahead.tiles;
-      a_there = next_item<F::kRows>(a, c.kv_heads, most, ahead);
-    }
-    if (a_there) {
-      const int tile = (int)(a_unit - a_first);
-      a_page = tile * kKv4Tile < ahead.len
-                   ? __ldg(a.block_table + ahead.b * a.table_stride + (tile >> per_page))
-                   : -2;  // a row tile that sees nothing
-    }
-  };
-  auto ahead_issue = [&](int stage) {
-    held &= ~(1u << stage);
-    if (!a_there) return;
-    if (a_page >= 0 && a_page < c.num_pages) {
-      held |= 1u << stage;
-      if (lane == 0) {
-        const int tile = (int)(a_unit - a_first);
-        bulk_load(smem_addr(ring + stage * F::kTile),
-                  c.base + (uint64_t)a_page * c.page_stride + (uint64_t)ahead.h * c.head_bytes +
-                      (uint64_t)(tile & ((1 << per_page) - 1)) * F::kTile,
-                  F::kTile, bars + 8 * stage);
+  // Pairs of tiles go round the warps across all items of the piece. `ahead` runs
+  // two pairs before the products; the lanes hold the pages of the next 16 pairs of
+  // the item, and a pair's two lanes fetch its tiles, whose presence is in `ok`.
+  Walk ahead = w;
+  int a_pair = warp, a_i = 0, a_page = -1;  // a_pair: in the item; pairs of warps before this one are skipped
+  uint32_t a_ok = 0, ok = 0;                // ok: two bits for each half of the ring
+  bool a_more = more;
+  auto ahead_pages = [&]() {
+    const int tile = ahead.t0 + 2 * (a_pair + kWarps * (lane >> 1)) + (lane & 1);
+    a_i = 0;
+    a_page = -1;
+    if (tile < ahead.t1 && tile * kKv4Tile < ahead.it.len) {  // else none, or a row tile that sees nothing
+      a_page = __ldg(a.block_table + ahead.it.b * a.table_stride + (tile >> per_page));
+      if (a_page < 0 || a_page >= c.num_pages) {
+        kv4_error(c.errors, kErrBounds);
+        a_page = -1;
       }
-    } else if (a_page != -2 && lane == 0) {
-      kv4_error(c.errors, kErrBounds);
     }
-    a_unit += kWarps;
-    ahead_find();
+    a_ok = __ballot_sync(0xffffffffu, a_page >= 0);
   };
-  ahead_find();
-#pragma unroll 1
-  for (int i = 0; i < F::kStages; ++i) ahead_issue(i);
+  auto ahead_item = [&]() {  // moves to the item that a_pair is in
+    while (a_more && a_pair >= (ahead.t1 - ahead.t0 + 1) / 2) {
+      a_pair -= (ahead.t1 - ahead.t0 + 1) / 2;
+      a_more = next_in_piece<F::kRows>(a, c.kv_heads, most, units, ahead);
+    }
+    if (a_more) ahead_pages();
+  };
+  auto ahead_issue = [&](int half) {
+    if (!a_more) return;
+    ok = half ? (ok & 3u) | (a_ok >> (2 * a_i) & 3u) << 2 : (ok & 12u) | (a_ok >> (2 * a_i) & 3u);
+    if ((lane >> 1) == a_i) {
+      const uint32_t bar = bars + 8 * half;
+      if (a_page >= 0) {
+        const int tile = ahead.t0 + 2 * a_pair + (lane & 1);
+        bulk_load(ring_at + (2 * half + (lane & 1)) * F::kTile,
+                  c.base + (uint64_t)a_page * c.page_stride + (uint64_t)ahead.it.h * c.head_bytes +
+                      (uint32_t)((tile & ((1 << per_page) - 1)) * F::kTile),
+                  F::kTile, bar);
+      } else {
+        asm volatile("mbarrier.arrive.shared.b64 _, [%0];" ::"r"(bar) : "memory");
+      }
+    }
+    a_pair += kWarps;
+    if (a_pair >= (ahead.t1 - ahead.t0 + 1) / 2) ahead_item();
+    else if (++a_i == 16) ahead_pages();
+  };
+  ahead_item();
+  ahead_issue(0);
+  ahead_issue(1);
 
-  int stage = 0;
-  long long unit = f0 + warp;
+  int half = 0, pair = warp;
+  uint32_t parity = 0;
   int4 join = make_int4(0, 0, 0, 0);
   bool first_segment = true;
-  for (long long seg = f0; seg < f1;) {
-    const long long end = min(first + it.tiles, f1);  // of this segment
-    const int rows = min(F::kRows, it.qn * a.ratio - it.rt * F::kRows);
+  for (; more; more = next_in_piece<F::kRows>(a, c.kv_heads, most, units, w)) {
+    const Item &it = w.it;
+    const int rows = min(F::kRows, it.qn * a.ratio - it.rt * F::kRows), pairs = (w.t1 - w.t0 + 1) / 2;
     // ---- the query rows: fp16 operands, their scale, their sums by group
 #pragma unroll 1
     for (int r = warp; r < F::kRows; r += kWarps) {
@@ -383,12 +433,11 @@ __global__ void __launch_bounds__(kThreads, Form<D, NG, NT>::kCtasPerSm)
         reinterpret_cast<__half *>(qs)[((((r / 8) * (D / 16) + step) * 32 + (r % 8) * 4 + d % 32 / 8) * 2 + (k & 1)) * 2 +
                                        (d & 1)] = v;
       }
-      const float s2 = a.scale * kLog2e;
       if (lane == 0) {
-        q_scale[r] = __uint_as_float((uint32_t)(24 - 14 + e + 127) << 23) * s2;
+        q_scale[r] = __uint_as_float((uint32_t)(24 - 14 + e + 127) << 23) * a.scale * kLog2e;
         limits[r] = row_limit(a, it, min(row, it.qn * a.ratio - 1));
       }
-      if (lane % (32 / NG) == 0) q_sum[lane / (32 / NG) * F::kRows + r] = sum * s2;
+      if (lane % (32 / NG) == 0) q_sum[lane / (32 / NG) * F::kRows + r] = sum * __uint_as_float((uint32_t)(14 - 24 - e + 127) << 23);
     }
     __syncthreads();
     uint32_t qf[F::kQRegs ? D / 16 : 1][2];
@@ -399,15 +448,34 @@ __global__ void __launch_bounds__(kThreads, Form<D, NG, NT>::kCtasPerSm)
         qf[i][0] = v.x, qf[i][1] = v.y;
       }
     }
+    // The tile loop asks shared memory for these only where registers are short.
+    constexpr bool kCache = NT * NG <= 2;
+    float2 qa_[kCache ? NT : 1], qb_[kCache ? NT : 1][NG];
+    auto q_scales = [&](int n) { return *reinterpret_cast<const float2 *>(q_scale + n * 8 + 2 * t); };
+    auto q_sums = [&](int n, int gi) { return *reinterpret_cast<const float2 *>(q_sum + gi * F::kRows + n * 8 + 2 * t); };
+    if constexpr (kCache) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        qa_[n] = q_scales(n);
+#pragma unroll
+        for (int gi = 0; gi < NG; ++gi) qb_[n][gi] = q_sums(n, gi);
+      }
+    }
     const int sees_least = limits[0], sees_most = limits[F::kRows - 1];
 
-    float o[D / 16][NT][4], z[NT][2][NG], l[NT][2], over[NT][2], sub[NT][2];
+    // z: sum of p * offset_v; u: sum of rounded p', taken by a product with ones
+    // (where registers are short it is part of z, taken from the rounded values)
+    float o[D / 16][NT][4], z[NT][2][NG], u[F::kOnes ? NT : 1][NG][2], l[NT][2], over[NT][2], sub[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
       for (int i = 0; i < D / 16; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[i][n][e] = 0.0f;
+      if constexpr (F::kOnes) {
+#pragma unroll
+        for (int gi = 0; gi < NG; ++gi) u[n][gi][0] = u[n][gi][1] = 0.0f;
+      }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         l[n][h] = 0.0f;
@@ -417,7 +485,7 @@ __global__ void __launch_bounds__(kThreads, Form<D, NG, NT>::kCtasPerSm)
         for (int gi = 0; gi < NG; ++gi) z[n][h][gi] = 0.0f;
       }
     }
-    auto recentre = [&]() {  // o += z, summed over the lanes that share a row
+    auto recentre = [&]() {  // o += z - 8 u; z is summed over the lanes that share a row
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -429,6 +497,10 @@ __global__ void __launch_bounds__(kThreads, Form<D, NG, NT>::kCtasPerSm)
             x += __shfl_xor_sync(0xffffffffu, x, 8);
             x += __shfl_xor_sync(0xffffffffu, x, 16);
             z[n][h][gi] = 0.0f;
+            if constexpr (F::kOnes) {
+              x = fmaf(-8.0f, u[n][gi][h], x);
+              u[n][gi][h] = 0.0f;
+            }
 #pragma unroll
             for (int i = gi * F::kGroupWords * 2; i < (gi + 1) * F::kGroupWords * 2; ++i) {
               o[i][n][h] = fmaf(x, 0x1p-24f, o[i][n][h]);
@@ -439,116 +511,160 @@ __global__ void __launch_bounds__(kThreads, Form<D, NG, NT>::kCtasPerSm)
 
     int since = 0;
 #pragma unroll 1
-    for (; unit < end; unit += kWarps) {
-      const int tile = (int)(unit - first);
-      if (held >> stage & 1) {
-        const uint8_t *buf = ring + stage * F::kTile;
-        if (!bar_wait(bars + 8 * stage, parity >> stage & 1)) kv4_error(c.errors, kErrTimeout);
-        parity ^= 1u << stage;
+    for (; pair < pairs; pair += kWarps) {
+      if (!bar_wait(bars + 8 * half, parity >> half & 1)) kv4_error(c.errors, kErrTimeout);
+      parity ^= 1u << half;
+      const uint32_t there = ok >> (2 * half) & 3u;
+      constexpr int J = F::kJoint;
+#pragma unroll 1
+      for (int j0 = 0; j0 < 2; j0 += J) {
+        const uint8_t *buf = ring + (2 * half + j0) * F::kTile;
         // ---- scores
-        float s[NT][4];
-        uint32_t par[2][NG];
+        float s[J][NT][4];
+        uint32_t par[J][2][NG];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) load_words<NG>(buf + 16 * D + (g + 8 * h) * NG * 4, par[h]);
+        for (int j = 0; j < J; ++j) {
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+          for (int h = 0; h < 2; ++h) load_words<NG>(buf + j * F::kTile + 16 * D + (g + 8 * h) * NG * 4, par[j][h]);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) s[n][e] = 0.0f;
-        uint32_t w0[F::kWpr], w1[F::kWpr];
-        float acc[NT][4];
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[j][n][e] = 0.0f;
+        }
+        uint32_t w0[J][F::kWpr], w1[J][F::kWpr];
+        float acc[J][NT][4];
 #pragma unroll
         for (int i = 0; i < F::kWords; ++i) {
           if (i % F::kWpr == 0) {
-            const uint8_t *p = buf + (i / F::kWpr) * 16 * 16 * F::kWpr + g * 16 * F::kWpr + t * 4 * F::kWpr;
-            load_words<F::kWpr>(p, w0);
-            load_words<F::kWpr>(p + 8 * 16 * F::kWpr, w1);
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+              const uint8_t *p =
+                  buf + j * F::kTile + (i / F::kWpr) * 16 * 16 * F::kWpr + g * 16 * F::kWpr + t * 4 * F::kWpr;
+              load_words<F::kWpr>(p, w0[j]);
+              load_words<F::kWpr>(p + 8 * 16 * F::kWpr, w1[j]);
+            }
           }
           if (i % F::kGroupWords == 0) {
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+            for (int j = 0; j < J; ++j)
 #pragma unroll
-              for (int e = 0; e < 4; ++e) acc[n][e] = 0.0f;
+              for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[j][n][e] = 0.0f;
           }
-          uint32_t x = w0[i % F::kWpr], y = w1[i % F::kWpr];
 #pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            const uint32_t a0 = x & 0x000f000fu, a1 = y & 0x000f000fu, a2 = x & 0x00f000f0u, a3 = y & 0x00f000f0u;
+          for (int hw = 0; hw < 2; ++hw) {
+            uint2 b[NT];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-              if constexpr (F::kQRegs) {
-                mma(acc[n], a0, a1, a2, a3, qf[2 * i + half][0], qf[2 * i + half][1]);
-              } else {
-                const uint2 b = reinterpret_cast<const uint2 *>(qs)[(n * (D / 16) + 2 * i + half) * 32 + lane];
-                mma(acc[n], a0, a1, a2, a3, b.x, b.y);
-              }
+              if constexpr (F::kQRegs) b[n] = make_uint2(qf[2 * i + hw][0], qf[2 * i + hw][1]);
+              else b[n] = reinterpret_cast<const uint2 *>(qs)[(n * (D / 16) + 2 * i + hw) * 32 + lane];
             }
-            x >>= 8, y >>= 8;
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+              const uint32_t x = w0[j][i % F::kWpr] >> (8 * hw), y = w1[j][i % F::kWpr] >> (8 * hw);
+              const uint32_t a0 = x & 0x000f000fu, a1 = y & 0x000f000fu, a2 = x & 0x00f000f0u, a3 = y & 0x00f000f0u;
+#pragma unroll
+              for (int n = 0; n < NT; ++n) mma(acc[j][n], a0, a1, a2, a3, b[n].x, b[n].y);
+            }
           }
           if (i % F::kGroupWords == F::kGroupWords - 1) {
             const int gi = i / F::kGroupWords;
-            const float s0 = kv4_scale(par[0][gi]), s1 = kv4_scale(par[1][gi]);
-            const float b0 = fmaf(-8.0f, s0, kv4_offset(par[0][gi])), b1 = fmaf(-8.0f, s1, kv4_offset(par[1][gi]));
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-              const float2 qa = *reinterpret_cast<const float2 *>(q_scale + n * 8 + 2 * t);
-              const float2 qb = *reinterpret_cast<const float2 *>(q_sum + gi * F::kRows + n * 8 + 2 * t);
-              s[n][0] += fmaf(s0, acc[n][0] * qa.x, b0 * qb.x);
-              s[n][1] += fmaf(s0, acc[n][1] * qa.y, b0 * qb.y);
-              s[n][2] += fmaf(s1, acc[n][2] * qa.x, b1 * qb.x);
-              s[n][3] += fmaf(s1, acc[n][3] * qa.y, b1 * qb.y);
+            for (int j = 0; j < J; ++j) {
+              const float s0 = kv4_scale(par[j][0][gi]), s1 = kv4_scale(par[j][1][gi]);
+              const float b0 = fmaf(-8.0f, s0, kv4_offset(par[j][0][gi]));
+              const float b1 = fmaf(-8.0f, s1, kv4_offset(par[j][1][gi]));
+#pragma unroll
+              for (int n = 0; n < NT; ++n) {
+                float2 qb;
+                if constexpr (kCache) qb = qb_[n][gi];
+                else qb = q_sums(n, gi);
+                s[j][n][0] = fmaf(s0, acc[j][n][0], fmaf(b0, qb.x, s[j][n][0]));
+                s[j][n][1] = fmaf(s0, acc[j][n][1], fmaf(b0, qb.y, s[j][n][1]));
+                s[j][n][2] = fmaf(s1, acc[j][n][2], fmaf(b1, qb.x, s[j][n][2]));
+                s[j][n][3] = fmaf(s1, acc[j][n][3], fmaf(b1, qb.y, s[j][n][3]));
+              }
             }
           }
         }
-        // ---- V: everything leaves the ring here, so that the next tile may come in
-        uint32_t vpar[2][NG], vw[2][F::kWords];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          load_words<NG>(buf + 16 * D + 64 * NG + (g + 8 * h) * NG * 4, vpar[h]);
+        for (int n = 0; n < NT; ++n) {
+          float2 qa;
+          if constexpr (kCache) qa = qa_[n];
+          else qa = q_scales(n);
 #pragma unroll
-          for (int sl = 0; sl < F::kSlabs; ++sl)
-            load_words<F::kWpr>(buf + 8 * D + ((sl * 2 + h) * 32 + lane) * 4 * F::kWpr, vw[h] + sl * F::kWpr);
+          for (int j = 0; j < J; ++j)
+            s[j][n][0] *= qa.x, s[j][n][1] *= qa.y, s[j][n][2] *= qa.x, s[j][n][3] *= qa.y;
         }
-        __syncwarp();
-        ahead_issue(stage);
+        // ---- V: everything leaves the ring here, so that the next pair may come in
+        uint32_t vpar[J][2][NG], vw[J][2][F::kWords];
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint8_t *p = buf + j * F::kTile;
+            load_words<NG>(p + 16 * D + 64 * NG + (g + 8 * h) * NG * 4, vpar[j][h]);
+#pragma unroll
+            for (int sl = 0; sl < F::kSlabs; ++sl)
+              load_words<F::kWpr>(p + 8 * D + ((sl * 2 + h) * 32 + lane) * 4 * F::kWpr, vw[j][h] + sl * F::kWpr);
+          }
+        const int tile = w.t0 + 2 * pair + j0;
+        if (j0 + J == 2) {
+          __syncwarp();
+          ahead_issue(half);
+        }
 
-        // ---- weights. Rows of tokens t0 + g and t0 + g + 8.
-        const int tok = tile * kKv4Tile + g;
-        const bool partial = (tile + 1) * kKv4Tile > sees_least;
+        // ---- weights. Rows of tokens t0 + g and t0 + g + 8 of each tile.
+        const bool partial = (tile + J) * kKv4Tile > sees_least || (there >> j0) != (J == 2 ? 3u : 3u >> j0);
         if (partial) {
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            const int2 lim = *reinterpret_cast<const int2 *>(limits + n * 8 + 2 * t);
-            s[n][0] = tok < lim.x ? s[n][0] : -INFINITY;
-            s[n][1] = tok < lim.y ? s[n][1] : -INFINITY;
-            s[n][2] = tok + 8 < lim.x ? s[n][2] : -INFINITY;
-            s[n][3] = tok + 8 < lim.y ? s[n][3] : -INFINITY;
-          }
+          for (int j = 0; j < J; ++j) {
+            const int tok = (there >> (j0 + j) & 1) ? (tile + j) * kKv4Tile + g : 0x7fffff00;  // a tile not there
 #pragma unroll
-          for (int gi = 0; gi < NG; ++gi) {
-            if (tok >= sees_most) vpar[0][gi] = 0;
-            if (tok + 8 >= sees_most) vpar[1][gi] = 0;
+            for (int n = 0; n < NT; ++n) {
+              const int2 lim = *reinterpret_cast<const int2 *>(limits + n * 8 + 2 * t);
+              s[j][n][0] = tok < lim.x ? s[j][n][0] : -INFINITY;
+              s[j][n][1] = tok < lim.y ? s[j][n][1] : -INFINITY;
+              s[j][n][2] = tok + 8 < lim.x ? s[j][n][2] : -INFINITY;
+              s[j][n][3] = tok + 8 < lim.y ? s[j][n][3] : -INFINITY;
+            }
+#pragma unroll
+            for (int gi = 0; gi < NG; ++gi) {
+              if (tok >= sees_most) vpar[j][0][gi] = 0;
+              if (tok + 8 >= sees_most) vpar[j][1][gi] = 0;
+            }
           }
         }
-        // p' = p * scale_v stays near 1 if the maximum is taken over s + log2 scale_v
-        float ev[2];
+        // p' = p * scale_v stays near 1 if the maximum is taken over s + log2
+        // scale_v (its exponent; a subnormal scale counts as 2^-15)
+        float ev[J][2];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float top = 0x1p-24f;
+        for (int j = 0; j < J; ++j)
 #pragma unroll
-          for (int gi = 0; gi < NG; ++gi) top = fmaxf(top, kv4_scale(vpar[h][gi]));
-          ev[h] = (float)((int)(__float_as_uint(top) >> 23) - 127);
-        }
+          for (int h = 0; h < 2; ++h) {
+            uint32_t top = 0;
+#pragma unroll
+            for (int gi = 0; gi < NG; ++gi) top = max(top, vpar[j][h][gi] & 0x7fffu);
+            ev[j][h] = (float)((int)(top >> 10) - 15);
+          }
+        float high[NT][2];
         bool raise = false;
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) raise |= s[n][e] + ev[e >> 1] > over[n][e & 1];
+          for (int h = 0; h < 2; ++h) {
+            high[n][h] = fmaxf(s[0][n][h] + ev[0][0], s[0][n][2 + h] + ev[0][1]);
+            if (J == 2)
+              high[n][h] = fmaxf(high[n][h], fmaxf(s[J - 1][n][h] + ev[J - 1][0], s[J - 1][n][2 + h] + ev[J - 1][1]));
+            raise |= high[n][h] > over[n][h];
+          }
         if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
           for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-              float m = fmaxf(s[n][h] + ev[0], s[n][2 + h] + ev[1]);
+              float m = high[n][h];
               m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 4));
               m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
               m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
@@ -559,7 +675,10 @@ __global__ void __launch_bounds__(kThreads, Form<D, NG, NT>::kCtasPerSm)
               over[n][h] = m + kSlack;
               l[n][h] *= f;
 #pragma unroll
-              for (int gi = 0; gi < NG; ++gi) z[n][h][gi] *= f;
+              for (int gi = 0; gi < NG; ++gi) {
+                z[n][h][gi] *= f;
+                if constexpr (F::kOnes) u[n][gi][h] *= f;
+              }
 #pragma unroll
               for (int i = 0; i < D / 16; ++i) {
                 o[i][n][h] *= f;
@@ -568,66 +687,79 @@ __global__ void __launch_bounds__(kThreads, Form<D, NG, NT>::kCtasPerSm)
             }
         }
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int j = 0; j < J; ++j)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            s[n][e] = ex2(s[n][e] - sub[n][e & 1]);
-            l[n][e & 1] += s[n][e];
-          }
+          for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              s[j][n][e] = ex2(s[j][n][e] - sub[n][e & 1]);
+              l[n][e & 1] += s[j][n][e];
+            }
         // ---- O += V P'
 #pragma unroll
-        for (int gi = 0; gi < NG; ++gi) {
-          const float s0 = kv4_scale(vpar[0][gi]), s1 = kv4_scale(vpar[1][gi]);
-          const float f0_ = kv4_offset(vpar[0][gi]), f1_ = kv4_offset(vpar[1][gi]);
-          uint32_t b[NT][2];
+        for (int j = 0; j < J; ++j)
 #pragma unroll
-          for (int n = 0; n < NT; ++n) {
-            float p0 = s[n][0] * s0, p1 = s[n][1] * s0, p2 = s[n][2] * s1, p3 = s[n][3] * s1;
-            float y0 = s[n][0] * f0_, y1 = s[n][1] * f0_, y2 = s[n][2] * f1_, y3 = s[n][3] * f1_;
-            if (partial) {  // a weight of 0 beside an infinite or NaN scale is nothing
-              if (s[n][0] == 0.0f) p0 = y0 = 0.0f;
-              if (s[n][1] == 0.0f) p1 = y1 = 0.0f;
-              if (s[n][2] == 0.0f) p2 = y2 = 0.0f;
-              if (s[n][3] == 0.0f) p3 = y3 = 0.0f;
+          for (int gi = 0; gi < NG; ++gi) {
+            const float s0 = kv4_scale(vpar[j][0][gi]), s1 = kv4_scale(vpar[j][1][gi]);
+            const float y0 = kv4_offset(vpar[j][0][gi]), y1 = kv4_offset(vpar[j][1][gi]);
+            uint32_t b[NT][2];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              const float *p = s[j][n];
+              float p0 = p[0] * s0, p1 = p[1] * s0, p2 = p[2] * s1, p3 = p[3] * s1;
+              if (partial) {  // a weight of 0 beside an infinite or NaN scale is nothing
+                if (p[0] == 0.0f) p0 = 0.0f;
+                if (p[1] == 0.0f) p1 = 0.0f;
+                if (p[2] == 0.0f) p2 = 0.0f;
+                if (p[3] == 0.0f) p3 = 0.0f;
+                if (p[0] != 0.0f) z[n][0][gi] = fmaf(p[0], y0, z[n][0][gi]);
+                if (p[1] != 0.0f) z[n][1][gi] = fmaf(p[1], y0, z[n][1][gi]);
+                if (p[2] != 0.0f) z[n][0][gi] = fmaf(p[2], y1, z[n][0][gi]);
+                if (p[3] != 0.0f) z[n][1][gi] = fmaf(p[3], y1, z[n][1][gi]);
+              } else {
+                z[n][0][gi] = fmaf(p[0], y0, fmaf(p[2], y1, z[n][0][gi]));
+                z[n][1][gi] = fmaf(p[1], y0, fmaf(p[3], y1, z[n][1][gi]));
+              }
+              const __half2 h0 = __floats2half2_rn(p0, p1), h1 = __floats2half2_rn(p2, p3);
+              b[n][0] = transpose8(*reinterpret_cast<const uint32_t *>(&h0));
+              b[n][1] = transpose8(*reinterpret_cast<const uint32_t *>(&h1));
+              if constexpr (F::kOnes) {
+                mma_sum(u[n][gi][0], u[n][gi][1], b[n][0], b[n][1]);
+              } else {
+                const float2 r0 = __half22float2(h0), r1 = __half22float2(h1);
+                z[n][0][gi] = fmaf(-8.0f, r0.x + r1.x, z[n][0][gi]);
+                z[n][1][gi] = fmaf(-8.0f, r0.y + r1.y, z[n][1][gi]);
+              }
             }
-            const __half2 h0 = __floats2half2_rn(p0, p1), h1 = __floats2half2_rn(p2, p3);
-            const float2 r0 = __half22float2(h0), r1 = __half22float2(h1);
-            z[n][0][gi] += (y0 + y2) - 8.0f * (r0.x + r1.x);
-            z[n][1][gi] += (y1 + y3) - 8.0f * (r0.y + r1.y);
-            b[n][0] = transpose8(*reinterpret_cast<const uint32_t *>(&h0));
-            b[n][1] = transpose8(*reinterpret_cast<const uint32_t *>(&h1));
+#pragma unroll
+            for (int i = gi * F::kGroupWords; i < (gi + 1) * F::kGroupWords; ++i)
+#pragma unroll
+              for (int hw = 0; hw < 2; ++hw) {
+                const uint32_t x = vw[j][0][i] >> (8 * hw), y = vw[j][1][i] >> (8 * hw);
+                const uint32_t a0 = x & 0x000f000fu, a1 = x & 0x00f000f0u, a2 = y & 0x000f000fu, a3 = y & 0x00f000f0u;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) mma(o[2 * i + hw][n], a0, a1, a2, a3, b[n][0], b[n][1]);
+              }
           }
-#pragma unroll
-          for (int i = gi * F::kGroupWords; i < (gi + 1) * F::kGroupWords; ++i) {
-            uint32_t x = vw[0][i], y = vw[1][i];
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-              const uint32_t a0 = x & 0x000f000fu, a1 = x & 0x00f000f0u, a2 = y & 0x000f000fu, a3 = y & 0x00f000f0u;
-#pragma unroll
-              for (int n = 0; n < NT; ++n) mma(o[2 * i + half][n], a0, a1, a2, a3, b[n][0], b[n][1]);
-              x >>= 8, y >>= 8;
-            }
-          }
-        }
-        // Codes are sums around 7.5 scale until they are centred; the tensor
-        // cores cut low bits off a sum, which would add up over a long row.
-        if (++since == kRecentre) {
-          recentre();
-          since = 0;
-        }
-      } else {
-        ahead_issue(stage);
       }
-      stage = stage + 1 == F::kStages ? 0 : stage + 1;
+      // Codes are sums around 7.5 scale until they are centred; the tensor cores
+      // cut low bits off a sum, which would add up over a long row.
+      if (++since == kRecentre) {
+        recentre();
+        since = 0;
+      }
+      half ^= 1;
     }
+    pair -= pairs;
     recentre();
 
     // ---- the eight warps' results, one n-tile at a time
-    const bool whole = seg == first && end == first + it.tiles;
+    const bool whole = w.t0 == 0 && w.t1 == it.tiles;
     float *part = a.parts + ((long long)blockIdx.x * 2 + (first_segment ? 0 : 1)) * F::kPart;
 #pragma unroll
-    for (int n = 0; n < NT; ++n) {
-      if (n) __syncthreads();
+    for (int nd = 0; nd < NT * F::kSlabs; ++nd) {
+      const int n = nd / F::kSlabs, d0 = nd % F::kSlabs * F::kMergeD;
+      if (nd) __syncthreads();
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         float sum = l[n][h];
@@ -636,9 +768,9 @@ __global__ void __launch_bounds__(kThreads, Form<D, NG, NT>::kCtasPerSm)
         sum += __shfl_xor_sync(0xffffffffu, sum, 16);
         float *to = merge + (warp * 8 + 2 * t + h) * F::kOutStride + g;
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) {
-          to[16 * i] = o[i][n][h] * 0x1p24f;
-          to[16 * i + 8] = o[i][n][2 + h] * 0x1p20f;
+        for (int i = 0; i < F::kMergeD / 16; ++i) {
+          to[16 * i] = o[d0 / 16 + i][n][h] * 0x1p24f;
+          to[16 * i + 8] = o[d0 / 16 + i][n][2 + h] * 0x1p20f;
         }
         if (g == 0) {
           merge_ml[(warp * 8 + 2 * t + h) * 2] = over[n][h] == -INFINITY && sum == 0.0f ? -INFINITY : sub[n][h];
@@ -650,34 +782,34 @@ __global__ void __launch_bounds__(kThreads, Form<D, NG, NT>::kCtasPerSm)
       if (r < rows) {
         float m = -INFINITY, sum = 0.0f, f[kWarps];
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) m = fmaxf(m, merge_ml[(w * 8 + warp) * 2]);
+        for (int k = 0; k < kWarps; ++k) m = fmaxf(m, merge_ml[(k * 8 + warp) * 2]);
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-          const float mw = merge_ml[(w * 8 + warp) * 2];
-          f[w] = mw == -INFINITY ? 0.0f : ex2(mw - m);
-          sum += mw == -INFINITY ? 0.0f : f[w] * merge_ml[(w * 8 + warp) * 2 + 1];
+        for (int k = 0; k < kWarps; ++k) {
+          const float mk = merge_ml[(k * 8 + warp) * 2];
+          f[k] = mk == -INFINITY ? 0.0f : ex2(mk - m);
+          sum += mk == -INFINITY ? 0.0f : f[k] * merge_ml[(k * 8 + warp) * 2 + 1];
         }
         const int row = it.rt * F::kRows + r;
         const int64_t at = (int64_t)(it.q0 + row / a.ratio) * a.q_heads + it.h * a.ratio + row % a.ratio;
         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
 #pragma unroll
-        for (int i = 0; i < D / 64; ++i) {
+        for (int i = 0; i < F::kMergeD / 64; ++i) {
           const int d = i * 64 + lane * 2;
           float x = 0.0f, y = 0.0f;
 #pragma unroll
-          for (int w = 0; w < kWarps; ++w) {
-            const float2 v = *reinterpret_cast<const float2 *>(merge + (w * 8 + warp) * F::kOutStride + d);
-            if (f[w] != 0.0f) x = fmaf(f[w], v.x, x), y = fmaf(f[w], v.y, y);
+          for (int k = 0; k < kWarps; ++k) {
+            const float2 v = *reinterpret_cast<const float2 *>(merge + (k * 8 + warp) * F::kOutStride + d);
+            if (f[k] != 0.0f) x = fmaf(f[k], v.x, x), y = fmaf(f[k], v.y, y);
           }
           if (!whole) {
-            *reinterpret_cast<float2 *>(part + r * D + d) = make_float2(x, y);
+            *reinterpret_cast<float2 *>(part + r * D + d0 + d) = make_float2(x, y);
           } else if (a.bf16) {
-            reinterpret_cast<__nv_bfloat162 *>(a.out)[(at * D + d) / 2] = __floats2bfloat162_rn(x * inv, y * inv);
+            reinterpret_cast<__nv_bfloat162 *>(a.out)[(at * D + d0 + d) / 2] = __floats2bfloat162_rn(x * inv, y * inv);
           } else {
-            reinterpret_cast<__half2 *>(a.out)[(at * D + d) / 2] = __floats2half2_rn(x * inv, y * inv);
+            reinterpret_cast<__half2 *>(a.out)[(at * D + d0 + d) / 2] = __floats2half2_rn(x * inv, y * inv);
           }
         }
-        if (lane == 0) {
+        if (lane == 0 && d0 == 0) {
           if (!whole) {
             part[F::kRows * D + 2 * r] = m;
             part[F::kRows * D + 2 * r + 1] = sum;
@@ -687,16 +819,11 @@ __global__ void __launch_bounds__(kThreads, Form<D, NG, NT>::kCtasPerSm)
         }
       }
     }
-    if (seg == first && end < first + it.tiles) {  // begun here, ended elsewhere
-      const long long last = (first + it.tiles - 1) / share;
+    if (w.t0 == 0 && w.t1 < it.tiles) {  // begun here, ended elsewhere
+      const long long last = (f0 + w.at + it.tiles - 1) / share;
       join = make_int4(it.b, it.rt, it.h, (int)(last - blockIdx.x + 1) * 2 + (first_segment ? 0 : 1));
     }
     first_segment = false;
-    seg = end;
-    if (seg < f1) {
-      first += it.tiles;
-      next_item<F::kRows>(a, c.kv_heads, most, it);
-    }
   }
   if (threadIdx.x == 0) a.joins[blockIdx.x] = join;
 }
@@ -711,7 +838,7 @@ __global__ void __launch_bounds__(D) attend_join_kernel(const Kv4View c, const A
   if (n == 0) return;
   Item it;
   it.b = join.x, it.rt = join.y, it.h = join.z;
-  load_request(a, (int)min((long long)a.columns * c.page_size, 0x7fffffffll), it.b, it.q0, it.qn, it.len);
+  load_request(a, a.columns * c.page_size, it.b, it.q0, it.qn, it.len);
   const int r = blockIdx.y, row = it.rt * tile_rows + r;
   if (row >= it.qn * a.ratio) return;
   const int size = tile_rows * (D + 2);
@@ -827,10 +954,12 @@ int check(const cb_kv4_cache *cache, const cb_kv4_attend_args *a, Kv4View *c) {
   if (a->q_heads % cache->kv_heads) return kv4_fail(CB_ERR_ARG, "cb_kv4_attend: q_heads is not a multiple of kv_heads");
   if (!a->q_start && a->total_q != a->requests)
     return kv4_fail(CB_ERR_ARG, "cb_kv4_attend: without q_start there is one row for each request");
-  if ((long long)a->columns * cache->page_size > 0x7fffffffll)
-    return kv4_fail(CB_ERR_ARG, "cb_kv4_attend: a row may not hold more than 2^31 - 1 tokens");
+  if ((long long)a->columns * cache->page_size > kKv4MostTokens)
+    return kv4_fail(CB_ERR_ARG, "cb_kv4_attend: a row may not hold more than 2^30 tokens");
   if (a->requests > 0 && a->total_q > 0 && (!a->q || !a->out || !a->block_table || !a->kv_lens))
     return kv4_fail(CB_ERR_ARG, "cb_kv4_attend: missing array");
+  if (reinterpret_cast<uintptr_t>(a->out) & 15)
+    return kv4_fail(CB_ERR_ARG, "cb_kv4_attend: out must be 16-byte aligned");
   return CB_OK;
 }
 
@@ -876,7 +1005,7 @@ extern "C" int cb_kv4_attend(const cb_kv4_cache *cache, const cb_kv4_attend_args
   a.ratio = args->q_heads / cache->kv_heads;
   a.causal = args->causal;
   a.bf16 = args->dtype == CB_KV4_BF16;
-  a.min_share = kWarps;
+  a.min_share = kItemCost + 2 * kWarps;
   const cudaError_t e = by_form(cache->head_dim, cache->head_dim / cache->group, l.rows / 8,
                                 [&](auto d, auto ng, auto nt) {
                                   return run_few<decltype(d)::value, decltype(ng)::value, decltype(nt)::value>(

@@ -621,6 +621,9 @@ def test_refusals_of_the_python_layer():
         cache.attend(0, q, table, lens, out=q)
     with pytest.raises(ValueError):
         cache.attend(0, q, table, lens, out=torch.empty_like(q).float())
+    odd = torch.empty(q.numel() + 1, dtype=q.dtype, device=DEV)[1:].view_as(q)
+    with pytest.raises(ValueError):
+        cache.attend(0, q, table, lens, out=odd)
     with pytest.raises(ValueError):
         cache.attend(0, q.clone().requires_grad_(), table, lens)
     with pytest.raises(cascade_cpp.CascadeError):
