@@ -13,11 +13,11 @@ namespace cb {
 namespace {
 
 // Row tiles of 8*NT rows (query row x query head of one KV head), tokens in
-// tiles of 16. A unit of work is one token tile of one item (request, row tile,
-// KV head); the units of all items, in that order, are one long line, and every
-// CTA takes an equal piece of it, whatever the lengths are. An item that ends
-// up in several CTAs leaves partial sums in the workspace, joined by a second
-// kernel in a fixed order.
+// tiles of 16. An item is (request, row tile, KV head); the token tiles of all
+// items, in that order, are one long line, and every WARP takes an equal piece of
+// it, whatever the lengths are: warps share nothing and never wait for one
+// another. An item that ends up in several warps leaves partial sums in the
+// workspace, joined by a second kernel in a fixed order.
 //
 // Tensor-core form (16x8x16, fp16 in, fp32 sums): the cache is the 16-row
 // operand of both products and the 8*NT query rows the 8-wide one, so that the
@@ -36,12 +36,14 @@ namespace {
 // largest, for bf16.
 constexpr int kWarps = 8, kThreads = kWarps * 32;
 constexpr int kRecentre = 4;      // pairs of tiles between centrings of the sums
-// What an item costs a CTA beside its tiles (query rows in, eight warps'
-// results joined), in tiles: it takes this much of the line too.
-constexpr int kItemCost = 12;
+// What an item costs a warp beside its tiles (query rows in, results out), in
+// tiles: it takes this much of the line too.
+constexpr int kItemCost = 8;
 constexpr float kSlack = 8.0f;    // p may reach 2^8 before the maximum is raised
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr uint32_t kWaitLimit = 1u << 24;
+constexpr int kJoinWarps = 8, kJoinThreads = kJoinWarps * 32;
+constexpr int kJoinNone = 0, kJoinFew = 1, kJoinMany = 2, kManyParts = 48;
 
 struct AttendArgs {
   const void *q;
@@ -49,10 +51,15 @@ struct AttendArgs {
   float *lse;
   const int32_t *block_table, *kv_lens, *q_start;
   int64_t table_stride, q_token_stride, q_head_stride;
-  float *parts;  // partial sums: two per CTA
-  int4 *joins;   // per CTA: (first row tile entry, parts) of an item it begins and does not end
+  float *parts;  // partial sums: two per piece
+  // Of the item that a piece begins and does not end: its first query row, row
+  // tile, head and rows; twice its number of parts, plus the place of its first;
+  // and how its parts are joined (kJoin*).
+  int4 *joins;
+  int *join_n;
+  uint8_t *join_how;
   float scale;
-  int32_t requests, columns, total_q, q_heads, ratio, causal, bf16, min_share;
+  int32_t requests, columns, total_q, q_heads, ratio, causal, bf16, q_vec, min_share;
 };
 
 // What an item is: request b, row tile rt, KV head h, and its token tiles.
@@ -75,15 +82,11 @@ struct Form {
   // 6.5 TB/s * 0.8 us / 148 = 35 KB.
   static constexpr int kJoint = NT == 1 ? 2 : 1;  // tiles whose products run side by side
   static constexpr int kCtasPerSm = NT == 1 && D <= 128 ? 2 : 1;
-  static constexpr bool kQRegs = NT == 1 && D <= 128 && NG == 1;
-  static constexpr bool kOnes = NT * NG <= 2;
-  static constexpr int kMergeD = D / kSlabs;        // dims joined at once
-  static constexpr int kOutStride = kMergeD + 4;    // two rows are 8 banks apart
-  static constexpr int kRing = kWarps * 4 * kTile;
+  static constexpr int kRing = 4 * kTile;           // of a warp, as are the next two
   static constexpr int kQ = NT * (D / 16) * 32 * 8;
   static constexpr int kConst = kRows * (2 + NG) * 4;
-  static constexpr int kMerge = kWarps * 8 * (kOutStride + 2) * 4;
-  static constexpr int kSmem = kRing + kQ + kMerge + kConst + kWarps * 16;
+  static constexpr int kWarp = (kRing + kQ + kConst + 16 + 127) / 128 * 128;
+  static constexpr int kSmem = kWarps * kWarp;
   static constexpr int kPart = kRows * (D + 2);     // floats of a partial result
 };
 
@@ -116,15 +119,6 @@ CB_D void mma(float *c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-// u0, u1 += the sum over 16 rows of the columns 2t, 2t + 1 of b.
-CB_D void mma_sum(float &u0, float &u1, uint32_t b0, uint32_t b1) {
-  [[maybe_unused]] float x, y;  // rows 8..15 of the product
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%6,%7,%6,%7}, {%4,%5}, {%0,%1,%8,%8};"
-      : "+f"(u0), "+f"(u1), "=f"(x), "=f"(y)
-      : "r"(b0), "r"(b1), "r"(0x3c003c00u), "r"(0u), "f"(0.0f));
 }
 
 CB_D uint32_t transpose8(uint32_t x) {
@@ -172,6 +166,20 @@ CB_D int row_limit(const AttendArgs &a, const Item &it, int r) {
   return a.causal ? it.len - (it.qn - 1 - r / a.ratio) : it.len;
 }
 
+// The row of out (and lse) of a request's row r.
+CB_D int64_t out_row(const AttendArgs &a, const Item &it, int r) {
+  return (int64_t)(it.q0 + r / a.ratio) * a.q_heads + it.h * a.ratio + r % a.ratio;
+}
+
+CB_D uint32_t pack2(int bf16, float lo, float hi) {
+  if (bf16) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&v);
+  }
+  const __half2 v = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t *>(&v);
+}
+
 template <int ROWS>
 CB_D void item_tiles(const AttendArgs &a, Item &it) {
   const int last = min((it.rt + 1) * ROWS, it.qn * a.ratio) - 1;
@@ -213,13 +221,13 @@ CB_D long long warp_sum(long long x) {
   return x;
 }
 
-// Finds this CTA's piece [f0, f1) of the line and the item that holds f0, which
-// begins at `first`. All threads return the same.
+// Finds the warp's piece [f0, f1) of the line and the item that holds f0, which
+// begins at `first`; false if there is nothing left for it. All threads of the
+// block call.
 template <int ROWS>
 CB_D bool find_piece(const AttendArgs &a, const Kv4View &c, int most, long long &share, long long &f0, long long &f1,
                      long long &first, Item &it) {
-  __shared__ long long sums[kWarps], at_s;
-  __shared__ int where;
+  __shared__ long long sums[kWarps], ends[kThreads];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   long long total = 0, mine = 0;
   for (int b = threadIdx.x; b < a.requests; b += kThreads) {
@@ -230,20 +238,21 @@ CB_D bool find_piece(const AttendArgs &a, const Kv4View &c, int most, long long 
   }
   total = warp_sum(total);
   if (lane == 0) sums[warp] = total;
-  if (threadIdx.x == 0) where = -1;
   __syncthreads();
   total = 0;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) total += sums[w];
-  share = max((total + gridDim.x - 1) / gridDim.x, (long long)a.min_share);
-  f0 = blockIdx.x * share;
+  const long long pieces = (long long)gridDim.x * kWarps;
+  share = max((total + pieces - 1) / pieces, (long long)a.min_share);
+  const long long block_last = ((long long)blockIdx.x * kWarps + kWarps - 1) * share;
+  f0 = ((long long)blockIdx.x * kWarps + warp) * share;
   f1 = min(f0 + share, total);
-  if (f0 >= f1) return false;
+  bool found = false;
   long long before = 0;
-  for (int b0 = 0; b0 < a.requests; b0 += kThreads) {
+  for (int b0 = 0; b0 < a.requests && before <= block_last; b0 += kThreads) {
     const int b = b0 + threadIdx.x;
-    if (a.requests > kThreads) mine = b < a.requests ? request_tiles<ROWS>(a, c.kv_heads, most, b) : 0;
-    else if (b >= a.requests) mine = 0;
+    if (b >= a.requests) mine = 0;
+    else if (a.requests > kThreads) mine = request_tiles<ROWS>(a, c.kv_heads, most, b);
     long long v = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -253,22 +262,27 @@ CB_D bool find_piece(const AttendArgs &a, const Kv4View &c, int most, long long 
     __syncthreads();
     if (lane == 31) sums[warp] = v;
     __syncthreads();
-    long long chunk = 0, at = before + v - mine;
+    long long chunk = 0;
+    v += before;
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) at += sums[w];
+      if (w < warp) v += sums[w];
       chunk += sums[w];
     }
-    if (at <= f0 && f0 < at + mine) {
-      where = b;
-      at_s = at;
+    ends[threadIdx.x] = v;
+    __syncthreads();
+    if (!found && f0 < before + chunk) {  // the first request that ends behind f0
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < kThreads / 32; ++i) n += ends[i * 32 + lane] <= f0;
+      n = __reduce_add_sync(0xffffffffu, n);
+      it.b = b0 + n;
+      first = n ? ends[n - 1] : before;
+      found = true;
     }
     before += chunk;
-    if (before > f0) break;  // the same for all threads
   }
-  __syncthreads();
-  it.b = where;
-  first = at_s;
+  if (!found || f0 >= f1) return false;
   load_request(a, most, it.b, it.q0, it.qn, it.len);
   for (it.rt = 0;; ++it.rt) {
     item_tiles<ROWS>(a, it);
@@ -281,11 +295,11 @@ CB_D bool find_piece(const AttendArgs &a, const Kv4View &c, int most, long long 
   return true;
 }
 
-// A CTA's piece of the line, item by item: the item and its tiles [t0, t1) in
+// A warp's piece of the line, item by item: the item and its tiles [t0, t1) in
 // the piece. Positions count from the piece's beginning.
 struct Walk {
   Item it;
-  int at;  // of the item's first tile; not positive if it began in an earlier CTA
+  int at;  // of the item's first tile; not positive if it began in an earlier piece
   int t0, t1;
   CB_D void cut(int units) {
     t0 = max(0, -at);
@@ -309,18 +323,17 @@ __global__ void __launch_bounds__(kThreads, Form<D, NG, NT>::kCtasPerSm)
     attend_few_kernel(const Kv4View c, const AttendArgs a) {
   using F = Form<D, NG, NT>;
   extern __shared__ __align__(128) uint8_t smem[];
-  uint32_t *qs = reinterpret_cast<uint32_t *>(smem + F::kRing);
-  float *merge = reinterpret_cast<float *>(smem + F::kRing + F::kQ);
-  float *merge_ml = merge + kWarps * 8 * F::kOutStride;
-  float *q_scale = reinterpret_cast<float *>(smem + F::kRing + F::kQ + F::kMerge);
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const uint8_t *ring = smem + warp * F::kWarp;
+  uint2 *qs = reinterpret_cast<uint2 *>(smem + warp * F::kWarp + F::kRing);
+  float *q_scale = reinterpret_cast<float *>(smem + warp * F::kWarp + F::kRing + F::kQ);
   int *limits = reinterpret_cast<int *>(q_scale + F::kRows);
   float *q_sum = reinterpret_cast<float *>(limits + F::kRows);  // [NG][rows]
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
-  const uint8_t *ring = smem + warp * 4 * F::kTile;
   const uint32_t ring_at = smem_addr(ring);
-  const uint32_t bars = smem_addr(smem + F::kRing + F::kQ + F::kMerge + F::kConst) + warp * 16;
+  const uint32_t bars = ring_at + F::kRing + F::kQ + F::kConst;
   const int most = a.columns * c.page_size;
   const int per_page = c.page_log2 - 4;
+  const int piece = blockIdx.x * kWarps + warp;
 
   asm volatile("griddepcontrol.launch_dependents;");
   if (lane == 0) {
@@ -332,7 +345,7 @@ __global__ void __launch_bounds__(kThreads, Form<D, NG, NT>::kCtasPerSm)
   long long share, f0, f1, first;
   Walk w;
   if (!find_piece<F::kRows>(a, c, most, share, f0, f1, first, w.it)) {
-    if (threadIdx.x == 0) a.joins[blockIdx.x] = make_int4(0, 0, 0, 0);
+    if (lane == 0) a.join_how[piece] = kJoinNone;
     return;
   }
   const int units = (int)(f1 - f0);
@@ -340,15 +353,15 @@ __global__ void __launch_bounds__(kThreads, Form<D, NG, NT>::kCtasPerSm)
   w.cut(units);
   bool more = w.t1 > w.t0 || next_in_piece<F::kRows>(a, c.kv_heads, most, units, w);
 
-  // Pairs of tiles go round the warps across all items of the piece. `ahead` runs
-  // two pairs before the products; the lanes hold the pages of the next 16 pairs of
-  // the item, and a pair's two lanes fetch its tiles, whose presence is in `ok`.
+  // `ahead` runs two pairs of tiles before the products; the lanes hold the pages of
+  // the next 16 pairs of the item, and a pair's two lanes fetch its tiles, whose
+  // presence is in `ok`.
   Walk ahead = w;
-  int a_pair = warp, a_i = 0, a_page = -1;  // a_pair: in the item; pairs of warps before this one are skipped
+  int a_tile = w.t0, a_i = 0, a_page = -1;
   uint32_t a_ok = 0, ok = 0;                // ok: two bits for each half of the ring
   bool a_more = more;
   auto ahead_pages = [&]() {
-    const int tile = ahead.t0 + 2 * (a_pair + kWarps * (lane >> 1)) + (lane & 1);
+    const int tile = a_tile + lane;
     a_i = 0;
     a_page = -1;
     if (tile < ahead.t1 && tile * kKv4Tile < ahead.it.len) {  // else none, or a row tile that sees nothing
@@ -360,94 +373,117 @@ __global__ void __launch_bounds__(kThreads, Form<D, NG, NT>::kCtasPerSm)
     }
     a_ok = __ballot_sync(0xffffffffu, a_page >= 0);
   };
-  auto ahead_item = [&]() {  // moves to the item that a_pair is in
-    while (a_more && a_pair >= (ahead.t1 - ahead.t0 + 1) / 2) {
-      a_pair -= (ahead.t1 - ahead.t0 + 1) / 2;
-      a_more = next_in_piece<F::kRows>(a, c.kv_heads, most, units, ahead);
-    }
-    if (a_more) ahead_pages();
-  };
   auto ahead_issue = [&](int half) {
     if (!a_more) return;
-    ok = half ? (ok & 3u) | (a_ok >> (2 * a_i) & 3u) << 2 : (ok & 12u) | (a_ok >> (2 * a_i) & 3u);
-    if ((lane >> 1) == a_i) {
+    ok = half ? (ok & 3u) | (a_ok >> a_i & 3u) << 2 : (ok & 12u) | (a_ok >> a_i & 3u);
+    const int j = lane - a_i;
+    if (j == 0 || j == 1) {
       const uint32_t bar = bars + 8 * half;
       if (a_page >= 0) {
-        const int tile = ahead.t0 + 2 * a_pair + (lane & 1);
-        bulk_load(ring_at + (2 * half + (lane & 1)) * F::kTile,
+        bulk_load(ring_at + (2 * half + j) * F::kTile,
                   c.base + (uint64_t)a_page * c.page_stride + (uint64_t)ahead.it.h * c.head_bytes +
-                      (uint32_t)((tile & ((1 << per_page) - 1)) * F::kTile),
+                      (uint32_t)(((a_tile + j) & ((1 << per_page) - 1)) * F::kTile),
                   F::kTile, bar);
       } else {
         asm volatile("mbarrier.arrive.shared.b64 _, [%0];" ::"r"(bar) : "memory");
       }
     }
-    a_pair += kWarps;
-    if (a_pair >= (ahead.t1 - ahead.t0 + 1) / 2) ahead_item();
-    else if (++a_i == 16) ahead_pages();
+    a_tile += 2;
+    a_i += 2;
+    if (a_tile >= ahead.t1) {
+      a_more = next_in_piece<F::kRows>(a, c.kv_heads, most, units, ahead);
+      a_tile = ahead.t0;
+      if (a_more) ahead_pages();
+    } else if (a_i == 32) {
+      ahead_pages();
+    }
   };
-  ahead_item();
+  if (a_more) ahead_pages();
   ahead_issue(0);
   ahead_issue(1);
 
-  int half = 0, pair = warp;
+  int half = 0;
   uint32_t parity = 0;
-  int4 join = make_int4(0, 0, 0, 0);
+  int how = kJoinNone;
   bool first_segment = true;
   for (; more; more = next_in_piece<F::kRows>(a, c.kv_heads, most, units, w)) {
     const Item &it = w.it;
-    const int rows = min(F::kRows, it.qn * a.ratio - it.rt * F::kRows), pairs = (w.t1 - w.t0 + 1) / 2;
-    // ---- the query rows: fp16 operands, their scale, their sums by group
+    const int rows = min(F::kRows, it.qn * a.ratio - it.rt * F::kRows);
+    // ---- the query rows as operands: fp16, their scale, their sums by group.
+    // A lane holds 8 dims of 32 of row g of each n-tile.
+    __syncwarp();
 #pragma unroll 1
-    for (int r = warp; r < F::kRows; r += kWarps) {
-      constexpr int kMine = D / 32;
-      float x[kMine];
-      float top = 0.0f;
-      const int row = it.rt * F::kRows + r;
-      if (r < rows) {
-        const int64_t at = (int64_t)(it.q0 + row / a.ratio) * a.q_token_stride +
-                           (int64_t)(it.h * a.ratio + row % a.ratio) * a.q_head_stride + lane * kMine;
+    for (int n = 0; n < NT; ++n) {
+      const int row = it.rt * F::kRows + n * 8 + g;
+      uint32_t x[F::kWords][4];
+      if (n * 8 + g < rows) {
+        const uint16_t *src = static_cast<const uint16_t *>(a.q) + (int64_t)(it.q0 + row / a.ratio) * a.q_token_stride +
+                              (int64_t)(it.h * a.ratio + row % a.ratio) * a.q_head_stride + 8 * t;
+        if (a.q_vec) {
 #pragma unroll
-        for (int i = 0; i < kMine; ++i) {
-          x[i] = a.bf16 ? kv4_load1(static_cast<const __nv_bfloat16 *>(a.q) + at + i)
-                        : kv4_load1(static_cast<const __half *>(a.q) + at + i);
-          top = fmaxf(top, fabsf(x[i]));
+          for (int i = 0; i < F::kWords; ++i) {
+            const uint4 v = __ldg(reinterpret_cast<const uint4 *>(src + 32 * i));
+            x[i][0] = v.x, x[i][1] = v.y, x[i][2] = v.z, x[i][3] = v.w;
+          }
+        } else {
+#pragma unroll
+          for (int i = 0; i < F::kWords; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k)
+              x[i][k] = __ldg(src + 32 * i + 2 * k) | (uint32_t)__ldg(src + 32 * i + 2 * k + 1) << 16;
         }
       } else {
 #pragma unroll
-        for (int i = 0; i < kMine; ++i) x[i] = 0.0f;
-      }
-      float sum = 0.0f;
+        for (int i = 0; i < F::kWords; ++i)
 #pragma unroll
-      for (int i = 0; i < kMine; ++i) sum += x[i];
-      for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      for (int o = 1; o < 32 / NG; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+          for (int k = 0; k < 4; ++k) x[i][k] = 0;
+      }
+      auto two = [&](uint32_t v) {
+        if (a.bf16) return make_float2(__uint_as_float(v << 16), __uint_as_float(v & 0xffff0000u));
+        return __half22float2(*reinterpret_cast<const __half2 *>(&v));
+      };
+      float top = 0.0f, sum[NG];
+#pragma unroll
+      for (int gi = 0; gi < NG; ++gi) sum[gi] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < F::kWords; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 v = two(x[i][k]);
+          top = fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y)));
+          sum[i / F::kGroupWords] += v.x + v.y;
+        }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
       // 2^(14 - e) with e the exponent of the largest; powers of two are exact
       const int e = min(max((int)(__float_as_uint(top) >> 23) - 127, -100), 110);
       const float up = __uint_as_float((uint32_t)(14 - e + 127) << 23);
+      const float down = __uint_as_float((uint32_t)(14 - 24 - e + 127) << 23);
 #pragma unroll
-      for (int i = 0; i < kMine; ++i) {
-        const int d = lane * kMine + i, k = d % 8 / 2;
-        const int step = d / 32 * 2 + k / 2;
-        const __half v = __float2half_rn(x[i] * up * (k & 1 ? 0.0625f : 1.0f));
-        reinterpret_cast<__half *>(qs)[((((r / 8) * (D / 16) + step) * 32 + (r % 8) * 4 + d % 32 / 8) * 2 + (k & 1)) * 2 +
-                                       (d & 1)] = v;
-      }
-      if (lane == 0) {
-        q_scale[r] = __uint_as_float((uint32_t)(24 - 14 + e + 127) << 23) * a.scale * kLog2e;
-        limits[r] = row_limit(a, it, min(row, it.qn * a.ratio - 1));
-      }
-      if (lane % (32 / NG) == 0) q_sum[lane / (32 / NG) * F::kRows + r] = sum * __uint_as_float((uint32_t)(14 - 24 - e + 127) << 23);
-    }
-    __syncthreads();
-    uint32_t qf[F::kQRegs ? D / 16 : 1][2];
-    if constexpr (F::kQRegs) {
+      for (int i = 0; i < F::kWords; ++i) {
+        uint32_t y[4];
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-        const uint2 v = reinterpret_cast<const uint2 *>(qs)[i * 32 + lane];
-        qf[i][0] = v.x, qf[i][1] = v.y;
+        for (int k = 0; k < 4; ++k) {
+          const float2 v = two(x[i][k]);
+          const float f = k & 1 ? up * 0.0625f : up;
+          const __half2 hv = __floats2half2_rn(v.x * f, v.y * f);
+          y[k] = *reinterpret_cast<const uint32_t *>(&hv);
+        }
+        qs[(n * (D / 16) + 2 * i) * 32 + lane] = make_uint2(y[0], y[1]);
+        qs[(n * (D / 16) + 2 * i + 1) * 32 + lane] = make_uint2(y[2], y[3]);
+      }
+#pragma unroll
+      for (int gi = 0; gi < NG; ++gi) {
+        sum[gi] += __shfl_xor_sync(0xffffffffu, sum[gi], 1);
+        sum[gi] += __shfl_xor_sync(0xffffffffu, sum[gi], 2);
+        if (t == 0) q_sum[gi * F::kRows + n * 8 + g] = sum[gi] * down;
+      }
+      if (t == 0) {
+        q_scale[n * 8 + g] = __uint_as_float((uint32_t)(24 - 14 + e + 127) << 23) * a.scale * kLog2e;
+        limits[n * 8 + g] = row_limit(a, it, min(row, it.qn * a.ratio - 1));
       }
     }
+    __syncwarp();
     // The tile loop asks shared memory for these only where registers are short.
     constexpr bool kCache = NT * NG <= 2;
     float2 qa_[kCache ? NT : 1], qb_[kCache ? NT : 1][NG];
@@ -463,19 +499,14 @@ __global__ void __launch_bounds__(kThreads, Form<D, NG, NT>::kCtasPerSm)
     }
     const int sees_least = limits[0], sees_most = limits[F::kRows - 1];
 
-    // z: sum of p * offset_v; u: sum of rounded p', taken by a product with ones
-    // (where registers are short it is part of z, taken from the rounded values)
-    float o[D / 16][NT][4], z[NT][2][NG], u[F::kOnes ? NT : 1][NG][2], l[NT][2], over[NT][2], sub[NT][2];
+    // z: sum of p * offset_v - 8 p', p' as rounded
+    float o[D / 16][NT][4], z[NT][2][NG], l[NT][2], over[NT][2], sub[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
       for (int i = 0; i < D / 16; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[i][n][e] = 0.0f;
-      if constexpr (F::kOnes) {
-#pragma unroll
-        for (int gi = 0; gi < NG; ++gi) u[n][gi][0] = u[n][gi][1] = 0.0f;
-      }
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         l[n][h] = 0.0f;
@@ -485,7 +516,7 @@ __global__ void __launch_bounds__(kThreads, Form<D, NG, NT>::kCtasPerSm)
         for (int gi = 0; gi < NG; ++gi) z[n][h][gi] = 0.0f;
       }
     }
-    auto recentre = [&]() {  // o += z - 8 u; z is summed over the lanes that share a row
+    auto recentre = [&]() {  // o += z, summed over the lanes that share a row
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -497,10 +528,6 @@ __global__ void __launch_bounds__(kThreads, Form<D, NG, NT>::kCtasPerSm)
             x += __shfl_xor_sync(0xffffffffu, x, 8);
             x += __shfl_xor_sync(0xffffffffu, x, 16);
             z[n][h][gi] = 0.0f;
-            if constexpr (F::kOnes) {
-              x = fmaf(-8.0f, u[n][gi][h], x);
-              u[n][gi][h] = 0.0f;
-            }
 #pragma unroll
             for (int i = gi * F::kGroupWords * 2; i < (gi + 1) * F::kGroupWords * 2; ++i) {
               o[i][n][h] = fmaf(x, 0x1p-24f, o[i][n][h]);
@@ -511,7 +538,7 @@ __global__ void __launch_bounds__(kThreads, Form<D, NG, NT>::kCtasPerSm)
 
     int since = 0;
 #pragma unroll 1
-    for (; pair < pairs; pair += kWarps) {
+    for (int tile0 = w.t0; tile0 < w.t1; tile0 += 2) {
       if (!bar_wait(bars + 8 * half, parity >> half & 1)) kv4_error(c.errors, kErrTimeout);
       parity ^= 1u << half;
       const uint32_t there = ok >> (2 * half) & 3u;
@@ -557,8 +584,7 @@ __global__ void __launch_bounds__(kThreads, Form<D, NG, NT>::kCtasPerSm)
             uint2 b[NT];
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-              if constexpr (F::kQRegs) b[n] = make_uint2(qf[2 * i + hw][0], qf[2 * i + hw][1]);
-              else b[n] = reinterpret_cast<const uint2 *>(qs)[(n * (D / 16) + 2 * i + hw) * 32 + lane];
+              b[n] = qs[(n * (D / 16) + 2 * i + hw) * 32 + lane];
             }
 #pragma unroll
             for (int j = 0; j < J; ++j) {
@@ -609,7 +635,7 @@ __global__ void __launch_bounds__(kThreads, Form<D, NG, NT>::kCtasPerSm)
             for (int sl = 0; sl < F::kSlabs; ++sl)
               load_words<F::kWpr>(p + 8 * D + ((sl * 2 + h) * 32 + lane) * 4 * F::kWpr, vw[j][h] + sl * F::kWpr);
           }
-        const int tile = w.t0 + 2 * pair + j0;
+        const int tile = tile0 + j0;
         if (j0 + J == 2) {
           __syncwarp();
           ahead_issue(half);
@@ -669,16 +695,13 @@ __global__ void __launch_bounds__(kThreads, Form<D, NG, NT>::kCtasPerSm)
               m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 8));
               m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 16));
               const bool fresh = over[n][h] == -INFINITY;
-              if (m == -INFINITY || (!fresh && m <= sub[n][h])) continue;
+              if (!(m > over[n][h])) continue;  // a row goes by its own scores; a NaN is no maximum
               const float f = fresh ? 1.0f : ex2(sub[n][h] - m);
               sub[n][h] = m;
               over[n][h] = m + kSlack;
               l[n][h] *= f;
 #pragma unroll
-              for (int gi = 0; gi < NG; ++gi) {
-                z[n][h][gi] *= f;
-                if constexpr (F::kOnes) u[n][gi][h] *= f;
-              }
+              for (int gi = 0; gi < NG; ++gi) z[n][h][gi] *= f;
 #pragma unroll
               for (int i = 0; i < D / 16; ++i) {
                 o[i][n][h] *= f;
@@ -723,13 +746,9 @@ __global__ void __launch_bounds__(kThreads, Form<D, NG, NT>::kCtasPerSm)
               const __half2 h0 = __floats2half2_rn(p0, p1), h1 = __floats2half2_rn(p2, p3);
               b[n][0] = transpose8(*reinterpret_cast<const uint32_t *>(&h0));
               b[n][1] = transpose8(*reinterpret_cast<const uint32_t *>(&h1));
-              if constexpr (F::kOnes) {
-                mma_sum(u[n][gi][0], u[n][gi][1], b[n][0], b[n][1]);
-              } else {
-                const float2 r0 = __half22float2(h0), r1 = __half22float2(h1);
-                z[n][0][gi] = fmaf(-8.0f, r0.x + r1.x, z[n][0][gi]);
-                z[n][1][gi] = fmaf(-8.0f, r0.y + r1.y, z[n][1][gi]);
-              }
+              const float2 r0 = __half22float2(h0), r1 = __half22float2(h1);
+              z[n][0][gi] = fmaf(-8.0f, r0.x + r1.x, z[n][0][gi]);
+              z[n][1][gi] = fmaf(-8.0f, r0.y + r1.y, z[n][1][gi]);
             }
 #pragma unroll
             for (int i = gi * F::kGroupWords; i < (gi + 1) * F::kGroupWords; ++i)
@@ -750,124 +769,193 @@ __global__ void __launch_bounds__(kThreads, Form<D, NG, NT>::kCtasPerSm)
       }
       half ^= 1;
     }
-    pair -= pairs;
     recentre();
 
-    // ---- the eight warps' results, one n-tile at a time
+    // ---- out: the result of an item that is all here, else a part of it
     const bool whole = w.t0 == 0 && w.t1 == it.tiles;
-    float *part = a.parts + ((long long)blockIdx.x * 2 + (first_segment ? 0 : 1)) * F::kPart;
+    float *part = a.parts + ((long long)piece * 2 + (first_segment ? 0 : 1)) * F::kPart;
 #pragma unroll
-    for (int nd = 0; nd < NT * F::kSlabs; ++nd) {
-      const int n = nd / F::kSlabs, d0 = nd % F::kSlabs * F::kMergeD;
-      if (nd) __syncthreads();
+    for (int n = 0; n < NT; ++n) {
+      float inv[2];
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         float sum = l[n][h];
         sum += __shfl_xor_sync(0xffffffffu, sum, 4);
         sum += __shfl_xor_sync(0xffffffffu, sum, 8);
         sum += __shfl_xor_sync(0xffffffffu, sum, 16);
-        float *to = merge + (warp * 8 + 2 * t + h) * F::kOutStride + g;
-#pragma unroll
-        for (int i = 0; i < F::kMergeD / 16; ++i) {
-          to[16 * i] = o[d0 / 16 + i][n][h] * 0x1p24f;
-          to[16 * i + 8] = o[d0 / 16 + i][n][2 + h] * 0x1p20f;
-        }
-        if (g == 0) {
-          merge_ml[(warp * 8 + 2 * t + h) * 2] = over[n][h] == -INFINITY && sum == 0.0f ? -INFINITY : sub[n][h];
-          merge_ml[(warp * 8 + 2 * t + h) * 2 + 1] = sum;
+        inv[h] = sum == 0.0f ? 0.0f : 1.0f / sum;
+        const int r = n * 8 + 2 * t + h;
+        if (g == 0 && whole) {
+          if (a.lse && r < rows)
+            a.lse[out_row(a, it, it.rt * F::kRows + r)] = sum == 0.0f ? -INFINITY : (sub[n][h] + log2f(sum)) * kLn2;
+        } else if (g == 0) {
+          reinterpret_cast<float2 *>(part + F::kRows * D)[r] =
+              make_float2(over[n][h] == -INFINITY && sum == 0.0f ? -INFINITY : sub[n][h], sum);
         }
       }
-      __syncthreads();
-      const int r = n * 8 + warp;
-      if (r < rows) {
-        float m = -INFINITY, sum = 0.0f, f[kWarps];
+      if (!whole) {
 #pragma unroll
-        for (int k = 0; k < kWarps; ++k) m = fmaxf(m, merge_ml[(k * 8 + warp) * 2]);
+        for (int i = 0; i < D / 16; ++i)
+          reinterpret_cast<float4 *>(part)[(n * (D / 16) + i) * 32 + lane] =
+              make_float4(o[i][n][0], o[i][n][1], o[i][n][2], o[i][n][3]);
+      } else {
+        // lanes g and g ^ 1 exchange, so that each stores two adjacent dims of one row
+        const int r = n * 8 + 2 * t + (g & 1);
+        uint32_t *to = static_cast<uint32_t *>(a.out) +
+                       (out_row(a, it, it.rt * F::kRows + min(r, rows - 1)) * D + (g & 6)) / 2;
 #pragma unroll
-        for (int k = 0; k < kWarps; ++k) {
-          const float mk = merge_ml[(k * 8 + warp) * 2];
-          f[k] = mk == -INFINITY ? 0.0f : ex2(mk - m);
-          sum += mk == -INFINITY ? 0.0f : f[k] * merge_ml[(k * 8 + warp) * 2 + 1];
-        }
-        const int row = it.rt * F::kRows + r;
-        const int64_t at = (int64_t)(it.q0 + row / a.ratio) * a.q_heads + it.h * a.ratio + row % a.ratio;
-        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        for (int i = 0; i < D / 16; ++i)
 #pragma unroll
-        for (int i = 0; i < F::kMergeD / 64; ++i) {
-          const int d = i * 64 + lane * 2;
-          float x = 0.0f, y = 0.0f;
-#pragma unroll
-          for (int k = 0; k < kWarps; ++k) {
-            const float2 v = *reinterpret_cast<const float2 *>(merge + (k * 8 + warp) * F::kOutStride + d);
-            if (f[k] != 0.0f) x = fmaf(f[k], v.x, x), y = fmaf(f[k], v.y, y);
+          for (int e = 0; e < 2; ++e) {
+            const float f = e ? 0x1p20f : 0x1p24f;
+            const float x = o[i][n][2 * e] * f * inv[0], y = o[i][n][2 * e + 1] * f * inv[1];
+            const float got = __shfl_xor_sync(0xffffffffu, g & 1 ? x : y, 4);
+            if (r < rows) to[(16 * i + 8 * e) / 2] = g & 1 ? pack2(a.bf16, got, y) : pack2(a.bf16, x, got);
           }
-          if (!whole) {
-            *reinterpret_cast<float2 *>(part + r * D + d0 + d) = make_float2(x, y);
-          } else if (a.bf16) {
-            reinterpret_cast<__nv_bfloat162 *>(a.out)[(at * D + d0 + d) / 2] = __floats2bfloat162_rn(x * inv, y * inv);
-          } else {
-            reinterpret_cast<__half2 *>(a.out)[(at * D + d0 + d) / 2] = __floats2half2_rn(x * inv, y * inv);
-          }
-        }
-        if (lane == 0 && d0 == 0) {
-          if (!whole) {
-            part[F::kRows * D + 2 * r] = m;
-            part[F::kRows * D + 2 * r + 1] = sum;
-          } else if (a.lse) {
-            a.lse[at] = sum == 0.0f ? -INFINITY : (m + log2f(sum)) * kLn2;
-          }
-        }
       }
     }
     if (w.t0 == 0 && w.t1 < it.tiles) {  // begun here, ended elsewhere
-      const long long last = (f0 + w.at + it.tiles - 1) / share;
-      join = make_int4(it.b, it.rt, it.h, (int)(last - blockIdx.x + 1) * 2 + (first_segment ? 0 : 1));
+      const int parts = (int)((f0 + w.at + it.tiles - 1) / share) - piece + 1;
+      how = parts > kManyParts ? kJoinMany : kJoinFew;
+      if (lane == 0) {
+        a.joins[piece] = make_int4(it.q0, it.rt, it.h, it.qn * a.ratio);
+        a.join_n[piece] = parts * 2 + (first_segment ? 0 : 1);
+      }
     }
     first_segment = false;
   }
-  if (threadIdx.x == 0) a.joins[blockIdx.x] = join;
+  if (lane == 0) a.join_how[piece] = (uint8_t)how;
 }
 
-// Joins the parts of the items that CTAs of the first kernel began and did not
-// end: block (x, r) does row r of CTA x's. Parts are taken in order.
+// Joins the parts of the items that a piece began and did not end, 16 dims of 8
+// rows (a chunk) at a time. A block does eight chunks of an item, a warp each, or
+// one chunk with all its warps where the item has many parts (a long request that
+// is alone). The order of the sums depends on the number of parts alone.
 template <int D>
-__global__ void __launch_bounds__(D) attend_join_kernel(const Kv4View c, const AttendArgs a, const int tile_rows) {
+__global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const AttendArgs a, const int pieces, const int nt) {
+  __shared__ int counts[kJoinWarps], task_s[3];
+  __shared__ float4 sums[kJoinWarps][32];
+  __shared__ float4 tops[kJoinWarps][4];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
+  const int chunks = nt * (D / 16), groups = (chunks + kJoinWarps - 1) / kJoinWarps;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int4 join = a.joins[blockIdx.x];
-  const int n = join.w >> 1;
-  if (n == 0) return;
-  Item it;
-  it.b = join.x, it.rt = join.y, it.h = join.z;
-  load_request(a, a.columns * c.page_size, it.b, it.q0, it.qn, it.len);
-  const int r = blockIdx.y, row = it.rt * tile_rows + r;
-  if (row >= it.qn * a.ratio) return;
-  const int size = tile_rows * (D + 2);
-  const float *one = a.parts + ((long long)blockIdx.x * 2 + (join.w & 1)) * size;
-  const float *rest = a.parts + ((long long)blockIdx.x * 2) * size;
-  float m = -INFINITY, sum = 0.0f, x = 0.0f;
-#pragma unroll 4
-  for (int i = 0; i < n; ++i) m = fmaxf(m, (i ? rest + (long long)i * 2 * size : one)[tile_rows * D + 2 * r]);
-#pragma unroll 4
-  for (int i = 0; i < n; ++i) {
-    const float *p = i ? rest + (long long)i * 2 * size : one;
-    const float mi = p[tile_rows * D + 2 * r], li = p[tile_rows * D + 2 * r + 1], v = p[r * D + threadIdx.x];
-    if (mi == -INFINITY) continue;
-    const float f = ex2(mi - m);
-    if (f != 0.0f) x = fmaf(f, v, x), sum = fmaf(f, li, sum);
+  // the blocks' tasks, in the order of the pieces; a thread counts 16 pieces
+  uint4 how = make_uint4(0, 0, 0, 0);
+  if (threadIdx.x * 16 < pieces) how = reinterpret_cast<const uint4 *>(a.join_how)[threadIdx.x];
+  const uint32_t words[4] = {how.x, how.y, how.z, how.w};
+  int mine = 0;
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    mine += __popc(words[k] & 0x01010101u * kJoinFew) * groups + __popc(words[k] & 0x01010101u * kJoinMany) * chunks;
+  int v = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += y;
   }
-  const int64_t at = (int64_t)(it.q0 + row / a.ratio) * a.q_heads + it.h * a.ratio + row % a.ratio;
-  x = sum == 0.0f ? 0.0f : x / sum;
-  if (a.bf16) static_cast<__nv_bfloat16 *>(a.out)[at * D + threadIdx.x] = __float2bfloat16_rn(x);
-  else static_cast<__half *>(a.out)[at * D + threadIdx.x] = __float2half_rn(x);
-  if (a.lse && threadIdx.x == 0) a.lse[at] = sum == 0.0f ? -INFINITY : (m + log2f(sum)) * kLn2;
+  if (lane == 31) counts[warp] = v;
+  __syncthreads();
+  int tasks = 0, begin = v - mine;
+#pragma unroll
+  for (int w = 0; w < kJoinWarps; ++w) {
+    if (w < warp) begin += counts[w];
+    tasks += counts[w];
+  }
+  const int part = nt * 8 * (D + 2);
+  for (int task = blockIdx.x; task < tasks; task += gridDim.x) {
+    __syncthreads();
+    if (task >= begin && task < begin + mine) {
+      int at = task - begin;
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        const int h = words[k / 4] >> (8 * (k % 4)) & 0xff, n = h == kJoinFew ? groups : h == kJoinMany ? chunks : 0;
+        if (at >= 0 && at < n) task_s[0] = threadIdx.x * 16 + k, task_s[1] = at, task_s[2] = h;
+        at -= n;
+      }
+    }
+    __syncthreads();
+    const int p = task_s[0], team = task_s[2] == kJoinMany ? kJoinWarps : 1;
+    const int chunk = team > 1 ? task_s[1] : task_s[1] * kJoinWarps + warp, n = chunk / (D / 16), i = chunk % (D / 16);
+    const int4 join = a.joins[p];
+    const int places = a.join_n[p], parts = places >> 1;
+    Item it;
+    it.q0 = join.x, it.rt = join.y, it.h = join.z;
+    const int rows = join.w - (it.rt * nt + n) * 8;
+    const bool here = chunk < chunks && rows > 0;
+    float4 m = make_float4(-INFINITY, 0.0f, -INFINITY, 0.0f);  // maximum and sum of rows 2t, 2t + 1
+    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    auto add = [](float &m, float &l, float &x, float &y, float mk, float lk, float xk, float yk) {
+      if (mk == -INFINITY) return;
+      const float top = fmaxf(m, mk);
+      const float f = m == -INFINITY ? 0.0f : ex2(m - top), fk = ex2(mk - top);
+      m = top;
+      l = l * f + lk * fk;
+      x = x * f + xk * fk;
+      y = y * f + yk * fk;
+    };
+    if (here) {
+      const float *base = a.parts + (long long)p * 2 * part;
+      constexpr int kBatch = 8;
+      for (int k0 = team > 1 ? warp : 0; k0 < parts; k0 += kBatch * team) {
+        float4 vs[kBatch], ms[kBatch];
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+          const int at = k0 + k * team;
+          ms[k] = make_float4(-INFINITY, 0.0f, -INFINITY, 0.0f);
+          if (at < parts) {
+            const float *from = base + (long long)at * 2 * part + (at ? 0 : (places & 1) * part);
+            vs[k] = reinterpret_cast<const float4 *>(from)[chunk * 32 + lane];
+            ms[k] = reinterpret_cast<const float4 *>(from + nt * 8 * D)[n * 4 + t];
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < kBatch; ++k) {
+          add(m.x, m.y, x.x, x.z, ms[k].x, ms[k].y, vs[k].x, vs[k].z);
+          add(m.z, m.w, x.y, x.w, ms[k].z, ms[k].w, vs[k].y, vs[k].w);
+        }
+      }
+    }
+    if (team > 1) {
+      sums[warp][lane] = x;
+      if (g == 0) tops[warp][t] = m;
+      __syncthreads();
+      if (warp == 0) {
+#pragma unroll
+        for (int w = 1; w < kJoinWarps; ++w) {
+          const float4 mw = tops[w][t], vw = sums[w][lane];
+          add(m.x, m.y, x.x, x.z, mw.x, mw.y, vw.x, vw.z);
+          add(m.z, m.w, x.y, x.w, mw.z, mw.w, vw.y, vw.w);
+        }
+      }
+    }
+    if (here && (team == 1 || warp == 0)) {
+      const int row = (it.rt * nt + n) * 8;
+      const float i0 = m.y == 0.0f ? 0.0f : 1.0f / m.y, i1 = m.w == 0.0f ? 0.0f : 1.0f / m.w;
+      if (i == 0 && g == 0 && a.lse) {
+        if (2 * t < rows) a.lse[out_row(a, it, row + 2 * t)] = m.y == 0.0f ? -INFINITY : (m.x + log2f(m.y)) * kLn2;
+        if (2 * t + 1 < rows)
+          a.lse[out_row(a, it, row + 2 * t + 1)] = m.w == 0.0f ? -INFINITY : (m.z + log2f(m.w)) * kLn2;
+      }
+      const int r = 2 * t + (g & 1);
+      uint32_t *to =
+          static_cast<uint32_t *>(a.out) + (out_row(a, it, row + min(r, rows - 1)) * D + 16 * i + (g & 6)) / 2;
+      const float x0 = x.x * 0x1p24f * i0, y0 = x.y * 0x1p24f * i1, x1 = x.z * 0x1p20f * i0, y1 = x.w * 0x1p20f * i1;
+      const float got0 = __shfl_xor_sync(0xffffffffu, g & 1 ? x0 : y0, 4);
+      const float got1 = __shfl_xor_sync(0xffffffffu, g & 1 ? x1 : y1, 4);
+      if (r < rows) {
+        to[0] = g & 1 ? pack2(a.bf16, got0, y0) : pack2(a.bf16, x0, got0);
+        to[4] = g & 1 ? pack2(a.bf16, got1, y1) : pack2(a.bf16, x1, got1);
+      }
+    }
+  }
 }
 
 // ------------------------------------------------------------------- the host
 
 struct Launch {
-  int rows;      // of a row tile
-  int ctas;
-  int part;      // floats of a partial result
+  int rows;  // of a row tile
+  int sms, ctas;
+  int part;  // floats of a partial result
 };
 
 constexpr int kMaxDevices = 64;
@@ -892,15 +980,15 @@ cudaError_t run_few(const Kv4View &c, const AttendArgs &a, const Launch &l, cuda
   attend_few_kernel<D, NG, NT><<<l.ctas, kThreads, F::kSmem, stream>>>(c, a);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(l.ctas, F::kRows);
-  cfg.blockDim = dim3(D);
+  cfg.gridDim = dim3(8 * l.sms);
+  cfg.blockDim = dim3(kJoinThreads);
   cfg.stream = stream;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, attend_join_kernel<D>, c, a, (int)F::kRows);
+  return cudaLaunchKernelEx(&cfg, attend_join_kernel<D>, a, l.ctas * kWarps, NT);
 }
 
 // f(integral constants D, NG, NT) for a cache and a number of n-tiles.
@@ -938,11 +1026,14 @@ Launch plan_launch(const cb_kv4_cache *cache, const cb_kv4_attend_args *a) {
   Launch l;
   l.rows = 8 * nt;
   l.part = l.rows * (cache->head_dim + 2);
-  l.ctas = sm_count(cache->device) * (nt == 1 && cache->head_dim <= 128 ? 2 : 1);
+  l.sms = min(sm_count(cache->device), kJoinThreads);  // a thread of the join counts 16 pieces
+  l.ctas = l.sms * (nt == 1 && cache->head_dim <= 128 ? 2 : 1);
   return l;
 }
 
-uint64_t workspace_bytes(const Launch &l) { return (uint64_t)l.ctas * (16 + 8ull * l.part); }
+uint64_t workspace_bytes(const Launch &l) { 
+  return (uint64_t)l.ctas * kWarps * (sizeof(int4) + 2ull * sizeof(float) * l.part + sizeof(int) + 1) + 16;
+}
 
 int check(const cb_kv4_cache *cache, const cb_kv4_attend_args *a, Kv4View *c) {
   if (!a) return kv4_fail(CB_ERR_ARG, "cb_kv4_attend: no arguments");
@@ -996,7 +1087,9 @@ extern "C" int cb_kv4_attend(const cb_kv4_cache *cache, const cb_kv4_attend_args
   a.q_token_stride = args->q_token_stride;
   a.q_head_stride = args->q_head_stride;
   a.joins = static_cast<int4 *>(args->workspace);
-  a.parts = reinterpret_cast<float *>(a.joins + l.ctas);
+  a.parts = reinterpret_cast<float *>(a.joins + l.ctas * kWarps);
+  a.join_n = reinterpret_cast<int *>(a.parts + (uint64_t)l.ctas * kWarps * 2 * l.part);
+  a.join_how = reinterpret_cast<uint8_t *>(a.join_n + l.ctas * kWarps);
   a.scale = args->scale;
   a.requests = args->requests;
   a.columns = args->columns;
@@ -1005,7 +1098,8 @@ extern "C" int cb_kv4_attend(const cb_kv4_cache *cache, const cb_kv4_attend_args
   a.ratio = args->q_heads / cache->kv_heads;
   a.causal = args->causal;
   a.bf16 = args->dtype == CB_KV4_BF16;
-  a.min_share = kItemCost + 2 * kWarps;
+  a.q_vec = ((reinterpret_cast<uintptr_t>(a.q) | (a.q_token_stride | a.q_head_stride) * 2) & 15) == 0;
+  a.min_share = kItemCost + 4;
   const cudaError_t e = by_form(cache->head_dim, cache->head_dim / cache->group, l.rows / 8,
                                 [&](auto d, auto ng, auto nt) {
                                   return run_few<decltype(d)::value, decltype(ng)::value, decltype(nt)::value>(
