@@ -43,7 +43,7 @@ constexpr float kSlack = 8.0f;    // p may reach 2^8 before the maximum is raise
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr uint32_t kWaitLimit = 1u << 24;
 constexpr int kJoinWarps = 8, kJoinThreads = kJoinWarps * 32;
-constexpr int kJoinNone = 0, kJoinFew = 1, kJoinMany = 2, kManyParts = 48;
+constexpr int kJoinNone = 0, kJoinFew = 1, kJoinMany = 2, kManyParts = 24;
 
 struct AttendArgs {
   const void *q;
@@ -133,6 +133,13 @@ CB_D float ex2(float x) {
   return y;
 }
 
+// A load that stays where it is written, before what waits for it.
+CB_D float4 load_now(const float *p) {
+  float4 v;
+  asm volatile("ld.global.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p) : "memory");
+  return v;
+}
+
 template <int N>
 CB_D void load_words(const uint8_t *p, uint32_t *w) {
   if constexpr (N == 1) w[0] = *reinterpret_cast<const uint32_t *>(p);
@@ -215,19 +222,39 @@ CB_D bool next_item(const AttendArgs &a, int heads, int most, Item &it) {
   return true;
 }
 
-CB_D long long warp_sum(long long x) {
+// a / b for b > 0, a >= 0, without the long division where both are short.
+CB_D long long quotient(long long a, int b) {
+  return a >> 31 ? a / b : (long long)((uint32_t)a / (uint32_t)b);
+}
+
+// Inclusive prefix sum over the block, and the block's sum. `sums` has an entry
+// for each warp and may not be in use.
+CB_D long long block_scan(long long v, long long *sums, long long &all) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
-  for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-  return x;
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long y = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += y;
+  }
+  if (lane == 31) sums[warp] = v;
+  __syncthreads();
+  all = 0;
+#pragma unroll
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) v += sums[w];
+    all += sums[w];
+  }
+  return v;
 }
 
 // Finds the warp's piece [f0, f1) of the line and the item that holds f0, which
-// begins at `first`; false if there is nothing left for it. All threads of the
-// block call.
+// begins at `first`; false if there is nothing left for it. Neighbouring pieces
+// are on different SMs, so that a short line is spread over all of them. All
+// threads of the block call.
 template <int ROWS>
 CB_D bool find_piece(const AttendArgs &a, const Kv4View &c, int most, long long &share, long long &f0, long long &f1,
                      long long &first, Item &it) {
-  __shared__ long long sums[kWarps], ends[kThreads];
+  __shared__ long long sums[2][kWarps], ends[kThreads];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   long long total = 0, mine = 0;
   for (int b = threadIdx.x; b < a.requests; b += kThreads) {
@@ -236,38 +263,20 @@ CB_D bool find_piece(const AttendArgs &a, const Kv4View &c, int most, long long 
     const int len = __ldg(a.kv_lens + b);
     if (blockIdx.x == 0 && (len < 0 || len > most)) kv4_error(c.errors, kErrBounds);
   }
-  total = warp_sum(total);
-  if (lane == 0) sums[warp] = total;
-  __syncthreads();
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) total += sums[w];
-  const long long pieces = (long long)gridDim.x * kWarps;
-  share = max((total + pieces - 1) / pieces, (long long)a.min_share);
-  const long long block_last = ((long long)blockIdx.x * kWarps + kWarps - 1) * share;
-  f0 = ((long long)blockIdx.x * kWarps + warp) * share;
+  const bool once = a.requests <= kThreads;  // a thread has a request at most
+  long long chunk, v = block_scan(total, sums[0], chunk);
+  total = chunk;
+  const int pieces = gridDim.x * kWarps;
+  share = max(quotient(total + pieces - 1, pieces), (long long)a.min_share);
+  f0 = (long long)(warp * gridDim.x + blockIdx.x) * share;
   f1 = min(f0 + share, total);
   bool found = false;
   long long before = 0;
-  for (int b0 = 0; b0 < a.requests && before <= block_last; b0 += kThreads) {
-    const int b = b0 + threadIdx.x;
-    if (b >= a.requests) mine = 0;
-    else if (a.requests > kThreads) mine = request_tiles<ROWS>(a, c.kv_heads, most, b);
-    long long v = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long y = __shfl_up_sync(0xffffffffu, v, o);
-      if (lane >= o) v += y;
-    }
-    __syncthreads();
-    if (lane == 31) sums[warp] = v;
-    __syncthreads();
-    long long chunk = 0;
-    v += before;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
-      if (w < warp) v += sums[w];
-      chunk += sums[w];
+  for (int b0 = 0; b0 < a.requests; b0 += kThreads) {
+    if (!once) {
+      const int b = b0 + threadIdx.x;
+      v = block_scan(b < a.requests ? request_tiles<ROWS>(a, c.kv_heads, most, b) : 0, sums[b0 / kThreads + 1 & 1],
+                     chunk) + before;
     }
     ends[threadIdx.x] = v;
     __syncthreads();
@@ -290,7 +299,7 @@ CB_D bool find_piece(const AttendArgs &a, const Kv4View &c, int most, long long 
     if (f0 < first + n) break;
     first += n;
   }
-  it.h = (int)((f0 - first) / (it.tiles + kItemCost));
+  it.h = (int)quotient(f0 - first, it.tiles + kItemCost);
   first += (long long)it.h * (it.tiles + kItemCost);
   return true;
 }
@@ -333,7 +342,7 @@ __global__ void __launch_bounds__(kThreads, Form<D, NG, NT>::kCtasPerSm)
   const uint32_t bars = ring_at + F::kRing + F::kQ + F::kConst;
   const int most = a.columns * c.page_size;
   const int per_page = c.page_log2 - 4;
-  const int piece = blockIdx.x * kWarps + warp;
+  const int piece = warp * gridDim.x + blockIdx.x;
 
   asm volatile("griddepcontrol.launch_dependents;");
   if (lane == 0) {
@@ -885,9 +894,8 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const AttendA
     float4 m = make_float4(-INFINITY, 0.0f, -INFINITY, 0.0f);  // maximum and sum of rows 2t, 2t + 1
     float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     auto add = [](float &m, float &l, float &x, float &y, float mk, float lk, float xk, float yk) {
-      if (mk == -INFINITY) return;
-      const float top = fmaxf(m, mk);
-      const float f = m == -INFINITY ? 0.0f : ex2(m - top), fk = ex2(mk - top);
+      const float top = fmaxf(m, mk), at = top == -INFINITY ? 0.0f : top;  // parts may hold nothing
+      const float f = ex2(m - at), fk = ex2(mk - at);
       m = top;
       l = l * f + lk * fk;
       x = x * f + xk * fk;
@@ -895,21 +903,19 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const AttendA
     };
     if (here) {
       const float *base = a.parts + (long long)p * 2 * part;
-      constexpr int kBatch = 8;
+      constexpr int kBatch = 4;
       for (int k0 = team > 1 ? warp : 0; k0 < parts; k0 += kBatch * team) {
         float4 vs[kBatch], ms[kBatch];
 #pragma unroll
         for (int k = 0; k < kBatch; ++k) {
-          const int at = k0 + k * team;
-          ms[k] = make_float4(-INFINITY, 0.0f, -INFINITY, 0.0f);
-          if (at < parts) {
-            const float *from = base + (long long)at * 2 * part + (at ? 0 : (places & 1) * part);
-            vs[k] = reinterpret_cast<const float4 *>(from)[chunk * 32 + lane];
-            ms[k] = reinterpret_cast<const float4 *>(from + nt * 8 * D)[n * 4 + t];
-          }
+          const int at = min(k0 + k * team, parts - 1);
+          const float *from = base + (long long)at * 2 * part + (at ? 0 : (places & 1) * part);
+          vs[k] = load_now(from + (chunk * 32 + lane) * 4);
+          ms[k] = load_now(from + nt * 8 * D + (n * 4 + t) * 4);
         }
 #pragma unroll
         for (int k = 0; k < kBatch; ++k) {
+          if (k0 + k * team >= parts) ms[k].x = ms[k].z = -INFINITY, ms[k].y = ms[k].w = 0.0f;
           add(m.x, m.y, x.x, x.z, ms[k].x, ms[k].y, vs[k].x, vs[k].z);
           add(m.z, m.w, x.y, x.w, ms[k].z, ms[k].w, vs[k].y, vs[k].w);
         }
@@ -1099,7 +1105,7 @@ extern "C" int cb_kv4_attend(const cb_kv4_cache *cache, const cb_kv4_attend_args
   a.causal = args->causal;
   a.bf16 = args->dtype == CB_KV4_BF16;
   a.q_vec = ((reinterpret_cast<uintptr_t>(a.q) | (a.q_token_stride | a.q_head_stride) * 2) & 15) == 0;
-  a.min_share = kItemCost + 4;
+  a.min_share = 2;
   const cudaError_t e = by_form(cache->head_dim, cache->head_dim / cache->group, l.rows / 8,
                                 [&](auto d, auto ng, auto nt) {
                                   return run_few<decltype(d)::value, decltype(ng)::value, decltype(nt)::value>(
