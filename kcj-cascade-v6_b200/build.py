@@ -18,7 +18,7 @@ BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "cascade_cpp", "libcascade_b200.so")
 
 SOURCES = ["sha256.cu", "copy.cu", "kvquant.cu", "index.cu", "store.cu", "pipeline.cu", "dht.cu", "policy.cpp",
-           "noalloc.cu", "kv4.cu", "kv4_attend.cu"]
+           "noalloc.cu", "kv4.cu", "kv4_attend.cu", "kv4_prompt.cu"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 
 

@@ -4,19 +4,15 @@
 //   out = sum_t p_t v_t / sum_t p_t,  p_t = exp(scale * q.k_t - max)
 //
 // in one pass over a row's tokens with the running maximum and sum.
-#include <type_traits>
-
-#include "kv4.cuh"
+#include "kv4_attend.cuh"
 
 namespace cb {
 
 namespace {
 
 // Row tiles of 8*NT rows (query row x query head of one KV head), tokens in
-// tiles of 16. An item is (request, row tile, KV head); the token tiles of all
-// items, in that order, are one long line, and every WARP takes an equal piece of
-// it, whatever the lengths are: warps share nothing and never wait for one
-// another. An item that ends up in several warps leaves partial sums in the
+// tiles of 16, a piece of the line (kv4_attend.cuh) for every WARP: warps share
+// nothing and never wait for one another. An item that ends up in several warps leaves partial sums in the
 // workspace, joined by a second kernel in a fixed order.
 //
 // Tensor-core form (16x8x16, fp16 in, fp32 sums): the cache is the 16-row
@@ -39,35 +35,8 @@ constexpr int kRecentre = 4;      // pairs of tiles between centrings of the sum
 // What an item costs a warp beside its tiles (query rows in, results out), in
 // tiles: it takes this much of the line too.
 constexpr int kItemCost = 8;
-constexpr float kSlack = 8.0f;    // p may reach 2^8 before the maximum is raised
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr uint32_t kWaitLimit = 1u << 24;
 constexpr int kJoinWarps = 8, kJoinThreads = kJoinWarps * 32;
-constexpr int kJoinNone = 0, kJoinFew = 1, kJoinMany = 2, kManyParts = 24;
-
-struct AttendArgs {
-  const void *q;
-  void *out;
-  float *lse;
-  const int32_t *block_table, *kv_lens, *q_start;
-  int64_t table_stride, q_token_stride, q_head_stride;
-  float *parts;  // partial sums: two per piece
-  // Of the item that a piece begins and does not end: its first query row, row
-  // tile, head and rows; twice its number of parts, plus the place of its first;
-  // and how its parts are joined (kJoin*).
-  int4 *joins;
-  int *join_n;
-  uint8_t *join_how;
-  float scale;
-  int32_t requests, columns, total_q, q_heads, ratio, causal, bf16, q_vec, min_share;
-};
-
-// What an item is: request b, row tile rt, KV head h, and its token tiles.
-struct Item {
-  int b, rt, h;
-  int q0, qn, len;  // the request's rows and tokens
-  int tiles;        // at least 1: a row tile that sees nothing still writes zeros
-};
+constexpr int kManyParts = 24;
 
 template <int D, int NG, int NT>
 struct Form {
@@ -88,24 +57,11 @@ struct Form {
   static constexpr int kWarp = (kRing + kQ + kConst + 16 + 127) / 128 * 128;
   static constexpr int kSmem = kWarps * kWarp;
   static constexpr int kPart = kRows * (D + 2);     // floats of a partial result
+  struct Line {
+    static constexpr int kRows = 8 * NT, kTokens = kKv4Tile, kCost = kItemCost, kWarps = cb::kWarps;
+    static constexpr bool kBlock = false;
+  };
 };
-
-CB_D uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
-CB_D void bar_init(uint32_t bar, uint32_t n) { asm volatile("mbarrier.init.shared.b64 [%0], %1;" ::"r"(bar), "r"(n)); }
-
-CB_D bool bar_wait(uint32_t bar, uint32_t parity) {
-  for (uint32_t i = 0; i < kWaitLimit; ++i) {
-    uint32_t ok;
-    asm volatile(
-        "{\n.reg .pred p;\nmbarrier.try_wait.parity.shared.b64 p, [%1], %2;\nselp.u32 %0, 1, 0, p;\n}"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    if (ok) return true;
-  }
-  return false;
-}
 
 CB_D void bulk_load(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar) {
   asm volatile("mbarrier.arrive.expect_tx.shared.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
@@ -127,12 +83,6 @@ CB_D uint32_t transpose8(uint32_t x) {
   return y;
 }
 
-CB_D float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
 // A load that stays where it is written, before what waits for it.
 CB_D float4 load_now(const float *p) {
   float4 v;
@@ -140,197 +90,11 @@ CB_D float4 load_now(const float *p) {
   return v;
 }
 
-template <int N>
-CB_D void load_words(const uint8_t *p, uint32_t *w) {
-  if constexpr (N == 1) w[0] = *reinterpret_cast<const uint32_t *>(p);
-  if constexpr (N == 2) {
-    const uint2 v = *reinterpret_cast<const uint2 *>(p);
-    w[0] = v.x, w[1] = v.y;
-  }
-  if constexpr (N >= 4) {
-#pragma unroll
-    for (int i = 0; i < N / 4; ++i) {
-      const uint4 v = *reinterpret_cast<const uint4 *>(p + 16 * i);
-      w[4 * i] = v.x, w[4 * i + 1] = v.y, w[4 * i + 2] = v.z, w[4 * i + 3] = v.w;
-    }
-  }
-}
-
-// The rows [q0, q0 + qn) of request b, inside [0, total_q), and its tokens.
-CB_D void load_request(const AttendArgs &a, int most, int b, int &q0, int &qn, int &len) {
-  if (!a.q_start) {
-    q0 = b;
-    qn = 1;
-  } else {
-    q0 = min(max(__ldg(a.q_start + b), 0), a.total_q);
-    qn = min(max(__ldg(a.q_start + b + 1), q0), a.total_q) - q0;
-  }
-  len = min(max(__ldg(a.kv_lens + b), 0), most);
-}
-
-// Tokens that row r (of qn * ratio) of a request sees.
-CB_D int row_limit(const AttendArgs &a, const Item &it, int r) {
-  return a.causal ? it.len - (it.qn - 1 - r / a.ratio) : it.len;
-}
-
-// The row of out (and lse) of a request's row r.
-CB_D int64_t out_row(const AttendArgs &a, const Item &it, int r) {
-  return (int64_t)(it.q0 + r / a.ratio) * a.q_heads + it.h * a.ratio + r % a.ratio;
-}
-
-CB_D uint32_t pack2(int bf16, float lo, float hi) {
-  if (bf16) {
-    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t *>(&v);
-  }
-  const __half2 v = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t *>(&v);
-}
-
-template <int ROWS>
-CB_D void item_tiles(const AttendArgs &a, Item &it) {
-  const int last = min((it.rt + 1) * ROWS, it.qn * a.ratio) - 1;
-  it.tiles = max(1, (row_limit(a, it, last) + kKv4Tile - 1) / kKv4Tile);
-}
-
-// What all items of request b take of the line.
-template <int ROWS>
-CB_D long long request_tiles(const AttendArgs &a, int heads, int most, int b) {
-  Item it;
-  load_request(a, most, b, it.q0, it.qn, it.len);
-  long long n = 0;
-  const int rts = (it.qn * a.ratio + ROWS - 1) / ROWS;
-  for (it.rt = 0; it.rt < rts; ++it.rt) {
-    item_tiles<ROWS>(a, it);
-    n += it.tiles + kItemCost;
-  }
-  return n * heads;
-}
-
-// The item behind `it`; false behind the last.
-template <int ROWS>
-CB_D bool next_item(const AttendArgs &a, int heads, int most, Item &it) {
-  if (++it.h < heads) return true;
-  it.h = 0;
-  ++it.rt;
-  while (it.rt * ROWS >= it.qn * a.ratio) {
-    it.rt = 0;
-    if (++it.b >= a.requests) return false;
-    load_request(a, most, it.b, it.q0, it.qn, it.len);
-  }
-  item_tiles<ROWS>(a, it);
-  return true;
-}
-
-// a / b for b > 0, a >= 0, without the long division where both are short.
-CB_D long long quotient(long long a, int b) {
-  return a >> 31 ? a / b : (long long)((uint32_t)a / (uint32_t)b);
-}
-
-// Inclusive prefix sum over the block, and the block's sum. `sums` has an entry
-// for each warp and may not be in use.
-CB_D long long block_scan(long long v, long long *sums, long long &all) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long y = __shfl_up_sync(0xffffffffu, v, o);
-    if (lane >= o) v += y;
-  }
-  if (lane == 31) sums[warp] = v;
-  __syncthreads();
-  all = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) v += sums[w];
-    all += sums[w];
-  }
-  return v;
-}
-
-// Finds the warp's piece [f0, f1) of the line and the item that holds f0, which
-// begins at `first`; false if there is nothing left for it. Neighbouring pieces
-// are on different SMs, so that a short line is spread over all of them. All
-// threads of the block call.
-template <int ROWS>
-CB_D bool find_piece(const AttendArgs &a, const Kv4View &c, int most, long long &share, long long &f0, long long &f1,
-                     long long &first, Item &it) {
-  __shared__ long long sums[2][kWarps], ends[kThreads];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  long long total = 0, mine = 0;
-  for (int b = threadIdx.x; b < a.requests; b += kThreads) {
-    mine = request_tiles<ROWS>(a, c.kv_heads, most, b);
-    total += mine;
-    const int len = __ldg(a.kv_lens + b);
-    if (blockIdx.x == 0 && (len < 0 || len > most)) kv4_error(c.errors, kErrBounds);
-  }
-  const bool once = a.requests <= kThreads;  // a thread has a request at most
-  long long chunk, v = block_scan(total, sums[0], chunk);
-  total = chunk;
-  const int pieces = gridDim.x * kWarps;
-  share = max(quotient(total + pieces - 1, pieces), (long long)a.min_share);
-  f0 = (long long)(warp * gridDim.x + blockIdx.x) * share;
-  f1 = min(f0 + share, total);
-  bool found = false;
-  long long before = 0;
-  for (int b0 = 0; b0 < a.requests; b0 += kThreads) {
-    if (!once) {
-      const int b = b0 + threadIdx.x;
-      v = block_scan(b < a.requests ? request_tiles<ROWS>(a, c.kv_heads, most, b) : 0, sums[b0 / kThreads + 1 & 1],
-                     chunk) + before;
-    }
-    ends[threadIdx.x] = v;
-    __syncthreads();
-    if (!found && f0 < before + chunk) {  // the first request that ends behind f0
-      int n = 0;
-#pragma unroll
-      for (int i = 0; i < kThreads / 32; ++i) n += ends[i * 32 + lane] <= f0;
-      n = __reduce_add_sync(0xffffffffu, n);
-      it.b = b0 + n;
-      first = n ? ends[n - 1] : before;
-      found = true;
-    }
-    before += chunk;
-  }
-  if (!found || f0 >= f1) return false;
-  load_request(a, most, it.b, it.q0, it.qn, it.len);
-  for (it.rt = 0;; ++it.rt) {
-    item_tiles<ROWS>(a, it);
-    const long long n = (long long)(it.tiles + kItemCost) * c.kv_heads;
-    if (f0 < first + n) break;
-    first += n;
-  }
-  it.h = (int)quotient(f0 - first, it.tiles + kItemCost);
-  first += (long long)it.h * (it.tiles + kItemCost);
-  return true;
-}
-
-// A warp's piece of the line, item by item: the item and its tiles [t0, t1) in
-// the piece. Positions count from the piece's beginning.
-struct Walk {
-  Item it;
-  int at;  // of the item's first tile; not positive if it began in an earlier piece
-  int t0, t1;
-  CB_D void cut(int units) {
-    t0 = max(0, -at);
-    t1 = min(it.tiles, units - at);
-  }
-};
-
-// The next item of the piece that has tiles in it; false behind the last.
-template <int ROWS>
-CB_D bool next_in_piece(const AttendArgs &a, int heads, int most, int units, Walk &w) {
-  do {
-    w.at += w.it.tiles + kItemCost;
-    if (w.at >= units || !next_item<ROWS>(a, heads, most, w.it)) return false;
-    w.cut(units);
-  } while (w.t1 <= w.t0);
-  return true;
-}
-
 template <int D, int NG, int NT>
 __global__ void __launch_bounds__(kThreads, Form<D, NG, NT>::kCtasPerSm)
     attend_few_kernel(const Kv4View c, const AttendArgs a) {
   using F = Form<D, NG, NT>;
+  using L = typename F::Line;
   extern __shared__ __align__(128) uint8_t smem[];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const uint8_t *ring = smem + warp * F::kWarp;
@@ -353,14 +117,15 @@ __global__ void __launch_bounds__(kThreads, Form<D, NG, NT>::kCtasPerSm)
   __syncwarp();
   long long share, f0, f1, first;
   Walk w;
-  if (!find_piece<F::kRows>(a, c, most, share, f0, f1, first, w.it)) {
+  __shared__ long long sums[2 * kWarps], ends[kThreads];
+  if (!find_piece<L>(a, c, most, sums, ends, share, f0, f1, first, w.it)) {
     if (lane == 0) a.join_how[piece] = kJoinNone;
     return;
   }
   const int units = (int)(f1 - f0);
-  w.at = (int)(first - f0) + kItemCost;
+  w.at = (int)(first - f0) + L::kCost;
   w.cut(units);
-  bool more = w.t1 > w.t0 || next_in_piece<F::kRows>(a, c.kv_heads, most, units, w);
+  bool more = w.t1 > w.t0 || next_in_piece<L>(a, c.kv_heads, most, units, w);
 
   // `ahead` runs two pairs of tiles before the products; the lanes hold the pages of
   // the next 16 pairs of the item, and a pair's two lanes fetch its tiles, whose
@@ -400,7 +165,7 @@ __global__ void __launch_bounds__(kThreads, Form<D, NG, NT>::kCtasPerSm)
     a_tile += 2;
     a_i += 2;
     if (a_tile >= ahead.t1) {
-      a_more = next_in_piece<F::kRows>(a, c.kv_heads, most, units, ahead);
+      a_more = next_in_piece<L>(a, c.kv_heads, most, units, ahead);
       a_tile = ahead.t0;
       if (a_more) ahead_pages();
     } else if (a_i == 32) {
@@ -415,7 +180,7 @@ __global__ void __launch_bounds__(kThreads, Form<D, NG, NT>::kCtasPerSm)
   uint32_t parity = 0;
   int how = kJoinNone;
   bool first_segment = true;
-  for (; more; more = next_in_piece<F::kRows>(a, c.kv_heads, most, units, w)) {
+  for (; more; more = next_in_piece<L>(a, c.kv_heads, most, units, w)) {
     const Item &it = w.it;
     const int rows = min(F::kRows, it.qn * a.ratio - it.rt * F::kRows);
     // ---- the query rows as operands: fp16, their scale, their sums by group.
@@ -958,12 +723,6 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const AttendA
 
 // ------------------------------------------------------------------- the host
 
-struct Launch {
-  int rows;  // of a row tile
-  int sms, ctas;
-  int part;  // floats of a partial result
-};
-
 constexpr int kMaxDevices = 64;
 
 int sm_count(int device) {
@@ -983,7 +742,7 @@ cudaError_t run_few(const Kv4View &c, const AttendArgs &a, const Launch &l, cuda
   cudaError_t e =
       cudaFuncSetAttribute(attend_few_kernel<D, NG, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem);
   if (e != cudaSuccess) return e;
-  attend_few_kernel<D, NG, NT><<<l.ctas, kThreads, F::kSmem, stream>>>(c, a);
+  attend_few_kernel<D, NG, NT><<<l.pieces / kWarps, kThreads, F::kSmem, stream>>>(c, a);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(8 * l.sms);
@@ -994,7 +753,7 @@ cudaError_t run_few(const Kv4View &c, const AttendArgs &a, const Launch &l, cuda
   at[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, attend_join_kernel<D>, a, l.ctas * kWarps, NT);
+  return cudaLaunchKernelEx(&cfg, attend_join_kernel<D>, a, l.pieces, NT);
 }
 
 // f(integral constants D, NG, NT) for a cache and a number of n-tiles.
@@ -1026,19 +785,29 @@ int few_tiles(int head_dim, int64_t rows) {
   return rows <= 16 || head_dim > 128 ? 2 : 4;
 }
 
-Launch plan_launch(const cb_kv4_cache *cache, const cb_kv4_attend_args *a) {
-  const int64_t ratio = a->q_heads / cache->kv_heads;
-  const int nt = few_tiles(cache->head_dim, ratio * (a->max_q > 1 ? a->max_q : 1));
-  Launch l;
-  l.rows = 8 * nt;
-  l.part = l.rows * (cache->head_dim + 2);
-  l.sms = min(sm_count(cache->device), kJoinThreads);  // a thread of the join counts 16 pieces
-  l.ctas = l.sms * (nt == 1 && cache->head_dim <= 128 ? 2 : 1);
-  return l;
-}
+// Above this many rows of a request the prompt kernel takes it (where it is
+// offered: head_dim 64 and 128); the few-row kernel would read the cache once for
+// every 32 rows.
+constexpr int kFewRows = 32;
 
-uint64_t workspace_bytes(const Launch &l) { 
-  return (uint64_t)l.ctas * kWarps * (sizeof(int4) + 2ull * sizeof(float) * l.part + sizeof(int) + 1) + 16;
+struct Launches {
+  Launch few, prompt;
+  bool prompts;  // whether a request may have more than kFewRows rows
+};
+
+Launches plan_launches(const cb_kv4_cache *cache, const cb_kv4_attend_args *a) {
+  const int64_t ratio = a->q_heads / cache->kv_heads, rows = ratio * (a->max_q > 1 ? a->max_q : 1);
+  const int d = cache->head_dim;
+  Launches l = {};
+  l.prompts = d <= 128 && rows > kFewRows;
+  // beside prompt chunks the others are single tokens in the main
+  const int nt = few_tiles(d, l.prompts ? ratio : rows);
+  l.few.sms = min(sm_count(cache->device) & ~1, kJoinThreads);  // a thread of the join counts 16 pieces
+  l.few.rows = 8 * nt;
+  l.few.part = l.few.rows * (d + 2);
+  l.few.pieces = l.few.sms * (nt == 1 && d <= 128 ? 2 : 1) * kWarps;
+  if (l.prompts) l.prompt = prompt_launch(d, l.few.sms);
+  return l;
 }
 
 int check(const cb_kv4_cache *cache, const cb_kv4_attend_args *a, Kv4View *c) {
@@ -1049,6 +818,7 @@ int check(const cb_kv4_cache *cache, const cb_kv4_attend_args *a, Kv4View *c) {
   if (a->requests < 0 || a->columns <= 0 || a->total_q < 0 || a->q_heads <= 0 || a->table_stride < a->columns)
     return kv4_fail(CB_ERR_ARG, "cb_kv4_attend: bad sizes");
   if (a->q_heads % cache->kv_heads) return kv4_fail(CB_ERR_ARG, "cb_kv4_attend: q_heads is not a multiple of kv_heads");
+  if ((long long)a->total_q * a->q_heads > 0x3fffffffll) return kv4_fail(CB_ERR_ARG, "cb_kv4_attend: too many rows");
   if (!a->q_start && a->total_q != a->requests)
     return kv4_fail(CB_ERR_ARG, "cb_kv4_attend: without q_start there is one row for each request");
   if ((long long)a->columns * cache->page_size > kKv4MostTokens)
@@ -1068,7 +838,8 @@ extern "C" uint64_t cb_kv4_attend_workspace(const cb_kv4_cache *cache, const cb_
   using namespace cb;
   Kv4View c;
   if (check(cache, a, &c) != CB_OK) return 0;
-  return workspace_bytes(plan_launch(cache, a));
+  const Launches l = plan_launches(cache, a);
+  return launch_bytes(l.few) + (l.prompts ? launch_bytes(l.prompt) : 0);
 }
 
 extern "C" int cb_kv4_attend(const cb_kv4_cache *cache, const cb_kv4_attend_args *args, void *stream) {
@@ -1076,8 +847,9 @@ extern "C" int cb_kv4_attend(const cb_kv4_cache *cache, const cb_kv4_attend_args
   Kv4View c;
   if (int rc = check(cache, args, &c)) return rc;
   if (args->requests == 0 || args->total_q == 0) return CB_OK;
-  const Launch l = plan_launch(cache, args);
-  if (!args->workspace || args->workspace_bytes < workspace_bytes(l) ||
+  const Launches l = plan_launches(cache, args);
+  const uint64_t need = launch_bytes(l.few) + (l.prompts ? launch_bytes(l.prompt) : 0);
+  if (!args->workspace || args->workspace_bytes < need ||
       (reinterpret_cast<uintptr_t>(args->workspace) & 15))
     return kv4_fail(CB_ERR_ARG, "cb_kv4_attend: workspace too small or not 16-byte aligned");
   Kv4Device dev(cache->device);
@@ -1092,10 +864,6 @@ extern "C" int cb_kv4_attend(const cb_kv4_cache *cache, const cb_kv4_attend_args
   a.table_stride = args->table_stride;
   a.q_token_stride = args->q_token_stride;
   a.q_head_stride = args->q_head_stride;
-  a.joins = static_cast<int4 *>(args->workspace);
-  a.parts = reinterpret_cast<float *>(a.joins + l.ctas * kWarps);
-  a.join_n = reinterpret_cast<int *>(a.parts + (uint64_t)l.ctas * kWarps * 2 * l.part);
-  a.join_how = reinterpret_cast<uint8_t *>(a.join_n + l.ctas * kWarps);
   a.scale = args->scale;
   a.requests = args->requests;
   a.columns = args->columns;
@@ -1105,11 +873,23 @@ extern "C" int cb_kv4_attend(const cb_kv4_cache *cache, const cb_kv4_attend_args
   a.causal = args->causal;
   a.bf16 = args->dtype == CB_KV4_BF16;
   a.q_vec = ((reinterpret_cast<uintptr_t>(a.q) | (a.q_token_stride | a.q_head_stride) * 2) & 15) == 0;
-  a.min_share = 2;
-  const cudaError_t e = by_form(cache->head_dim, cache->head_dim / cache->group, l.rows / 8,
-                                [&](auto d, auto ng, auto nt) {
-                                  return run_few<decltype(d)::value, decltype(ng)::value, decltype(nt)::value>(
-                                      c, a, l, static_cast<cudaStream_t>(stream));
-                                });
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e = cudaSuccess;
+  if (l.prompts) {
+    launch_arrays(l.prompt, static_cast<char *>(args->workspace) + launch_bytes(l.few), a);
+    a.rows_above = kFewRows;
+    a.rows_most = 0x7fffffff;
+    a.min_share = 1;
+    e = run_prompt(c, a, cache->head_dim, cache->group, l.prompt, st);
+  }
+  if (e == cudaSuccess) {
+    launch_arrays(l.few, args->workspace, a);
+    a.rows_above = 0;
+    a.rows_most = l.prompts ? kFewRows : 0x7fffffff;
+    a.min_share = 2;
+    e = by_form(cache->head_dim, cache->head_dim / cache->group, l.few.rows / 8, [&](auto d, auto ng, auto nt) {
+      return run_few<decltype(d)::value, decltype(ng)::value, decltype(nt)::value>(c, a, l.few, st);
+    });
+  }
   return e == cudaSuccess ? CB_OK : kv4_fail(CB_ERR_CUDA, "cb_kv4_attend: launch", e);
 }
