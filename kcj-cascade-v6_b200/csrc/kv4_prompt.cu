@@ -29,7 +29,11 @@ namespace {
 constexpr int kTok = 128;         // tokens of a tile
 constexpr int kTileRows = 128;    // rows of a product
 constexpr int kSoftWarps = 8, kDeqWarps = 4, kMmaWarp = kSoftWarps + kDeqWarps;
-constexpr int kPromptWarps = kMmaWarp + 1, kPromptThreads = kPromptWarps * 32;
+constexpr int kPromptWarps = 16, kPromptThreads = kPromptWarps * 32;  // the last three only make up a warpgroup
+// Registers of a thread: 512 * 128 at launch, then for a softmax thread as many as
+// hold a row of scores.
+constexpr int kSoftRegs = 184, kDeqRegs = 88, kMmaRegs = 56;
+static_assert(256 * kSoftRegs + 128 * kDeqRegs + 128 * kMmaRegs <= kPromptThreads * 128, "registers");
 constexpr int kRaw = 3;           // cache tiles in a dequantising warp's ring
 constexpr int kTmemCols = 512;
 
@@ -69,27 +73,41 @@ CB_D void tc_commit(uint32_t bar) {
 }
 
 // Operands in shared memory: rows of 64 fp16 (128 bytes) along the axis that is
-// summed over, 16-byte chunks exchanged within 8 rows by their number.
-CB_D uint64_t operand(uint32_t addr) {
-  return (uint64_t)((addr & 0x3ffff) >> 4) | (1ull << 16) | ((uint64_t)(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+// summed over, 16-byte chunks exchanged within 8 rows by their number. A
+// descriptor's low word holds the address, its high word is the same for all.
+constexpr uint32_t kOperandHigh = (1024 >> 4) | (1u << 14) | (2u << 29);
+CB_D uint32_t operand_low(uint32_t addr) { return ((addr & 0x3ffff) >> 4) | (1u << 16); }
+
+__host__ __device__ constexpr uint32_t product_shape(int n) {
+  return (1u << 4) | (uint32_t)(n / 8) << 17 | (uint32_t)(kTileRows / 16) << 24;
 }
 
-__host__ __device__ constexpr uint32_t product_shape(int n) { return (1u << 4) | (uint32_t)(n / 8) << 17 | (uint32_t)(kTileRows / 16) << 24; }
-
-CB_D void product_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, bool add) {
+// d (+)= a b. What the one thread issues has to be in uniform registers: with all
+// operands known to be the same for the warp, a product of 16 steps' worth is
+// issued in a few cycles, from ordinary registers in about 100 (measured), more
+// than it takes to compute.
+template <bool ADD>
+CB_D void product_ss(uint32_t d, uint32_t a, uint32_t b, uint32_t shape) {
   asm volatile(
-      "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d), "l"(a), "l"(b), "r"(shape),
-      "r"((uint32_t)add)
+      "{\n.reg .pred p;\n.reg .b64 da, db;\nmov.b64 da, {%1, %4};\nmov.b64 db, {%2, %4};\nsetp.ne.u32 p, %5, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p;\n}" ::"r"(d), "r"(a), "r"(b), "r"(shape),
+      "n"(kOperandHigh), "n"((int)ADD)
       : "memory");
 }
-CB_D void product_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t shape, bool add) {
+CB_D void product_ts(uint32_t d, uint32_t a, uint32_t b, uint32_t shape, uint32_t add) {
   asm volatile(
-      "{\n.reg .pred p;\nsetp.ne.u32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d), "r"(a), "l"(b), "r"(shape),
-      "r"((uint32_t)add)
+      "{\n.reg .pred p;\n.reg .b64 db;\nmov.b64 db, {%2, %4};\nsetp.ne.u32 p, %5, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n}" ::"r"(d), "r"(a), "r"(b), "r"(shape),
+      "n"(kOperandHigh), "r"(add)
       : "memory");
 }
+CB_D bool elected() {
+  uint32_t one;
+  asm volatile("{\n.reg .pred p;\nelect.sync _|p, 0xffffffff;\nselp.u32 %0, 1, 0, p;\n}" : "=r"(one));
+  return one;
+}
+// The same value, known to be so for the whole warp.
+CB_D uint32_t uniform(uint32_t x) { return __reduce_or_sync(0xffffffffu, x); }
 
 CB_D void tmem_load32(uint32_t addr, float *v) {
   uint32_t *r = reinterpret_cast<uint32_t *>(v);
@@ -130,6 +148,28 @@ CB_D void arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared.b64 _, [%0
 
 // A wait of a whole warp, which goes one way for all of it.
 CB_D bool warp_wait(uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, bar_wait(bar, parity)); }
+
+// Two fp32 values in one 64-bit register.
+CB_D uint64_t pair(float x, float y) {
+  uint64_t v;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y));
+  return v;
+}
+CB_D float2 unpair(uint64_t v) {
+  float2 f;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+  return f;
+}
+CB_D uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t v;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v) : "l"(a), "l"(b), "l"(c));
+  return v;
+}
+CB_D uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t v;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+  return v;
+}
 
 CB_D __half2 as_half2(uint32_t x) { return *reinterpret_cast<const __half2 *>(&x); }
 CB_D uint32_t as_u32(__half2 x) { return *reinterpret_cast<const uint32_t *>(&x); }
@@ -196,6 +236,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
   int how = kJoinNone;
 
   if (warp < kSoftWarps) {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftRegs));
     // -------------------------------------------------------------- softmax
     const int x = warp >> 2, r = (warp & 3) * 32 + lane;
     const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // this warp's lanes of tensor memory
@@ -266,25 +307,22 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
           const uint4 bad = *reinterpret_cast<const uint4 *>(fl.bad);
           const int visible = limit - (w.t0 + j) * kTok;  // columns below it are seen
           const bool masked = __any_sync(0xffffffffu, visible < kTok) || there != kAllThere;
-          float v[2][32];
-          auto hide = [&](float *y, int ch) {
-            const uint32_t on = there >> (8 * ch);
+          float v[kTok];
 #pragma unroll
-            for (int k = 0; k < 32; ++k)
-              if (32 * ch + k >= visible || !(on >> (k / 16) & 1)) y[k] = -INFINITY;
-          };
-          // ---- the row's largest score
-          float top2 = -INFINITY, top3 = -INFINITY;
-          tmem_load32(s_at, v[0]);
+          for (int ch = 0; ch < 4; ++ch) tmem_load32(s_at + 32 * ch, v + 32 * ch);
+          tc_wait_ld();
+          if (masked) {
 #pragma unroll
-          for (int ch = 0; ch < 4; ++ch) {
-            tc_wait_ld();
-            float *y = v[ch & 1];
-            if (ch < 3) tmem_load32(s_at + 32 * (ch + 1), v[(ch + 1) & 1]);
-            if (masked) hide(y, ch);
-#pragma unroll
-            for (int k = 0; k < 32; k += 2) top2 = fmaxf(top2, y[k]), top3 = fmaxf(top3, y[k + 1]);
+            for (int k = 0; k < kTok; ++k)
+              if (k >= visible || !(there >> (8 * (k / 32) + k / 16 % 2) & 1)) v[k] = -INFINITY;
           }
+          // ---- the row's largest score
+          float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int k = 0; k < kTok; k += 8)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) tops[i] = fmaxf(tops[i], fmaxf(v[k + 2 * i], v[k + 2 * i + 1]));
+          const float top2 = fmaxf(tops[0], tops[1]), top3 = fmaxf(tops[2], tops[3]);
           const float m = fmaxf(top2, top3) * to_log2;
           float f = 1.0f;
           if (m > over) {
@@ -295,11 +333,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
           if (j > 0 && __any_sync(0xffffffffu, f != 1.0f)) {
 #pragma unroll 1
             for (int d = 0; d < D; d += 32) {
-              tmem_load32(o_at + d, v[0]);
+              float y[32];
+              tmem_load32(o_at + d, y);
               tc_wait_ld();
 #pragma unroll
-              for (int k = 0; k < 32; ++k) v[0][k] *= f;
-              tmem_store32(o_at + d, v[0]);
+              for (int k = 0; k < 32; ++k) y[k] *= f;
+              tmem_store32(o_at + d, y);
             }
           }
           l *= f;
@@ -311,26 +350,23 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
               if (left > 0 && (b[ch] & (left >= 32 ? 0xffffffffu : (1u << left) - 1))) l = NAN;
             }
           }
-          // ---- weights, P over the columns of S that have been read
-          float l2 = 0.0f;
-          tmem_load32(s_at, v[0]);
+          // ---- weights, P over the columns of S
+          const uint64_t by = pair(to_log2, to_log2), minus = pair(-sub, -sub);
+          uint64_t sums[2] = {0, 0};
 #pragma unroll
           for (int ch = 0; ch < 4; ++ch) {
-            tc_wait_ld();
-            float *y = v[ch & 1];
-            if (ch < 3) tmem_load32(s_at + 32 * (ch + 1), v[(ch + 1) & 1]);
-            if (masked) hide(y, ch);
             uint32_t p[16];
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
-              const float p0 = ex2(fmaf(y[2 * k], to_log2, -sub)), p1 = ex2(fmaf(y[2 * k + 1], to_log2, -sub));
-              l += p0;
-              l2 += p1;
+              const float2 y = unpair(fma2(pair(v[32 * ch + 2 * k], v[32 * ch + 2 * k + 1]), by, minus));
+              const float p0 = ex2(y.x), p1 = ex2(y.y);
+              sums[k & 1] = add2(sums[k & 1], pair(p0, p1));
               p[k] = as_u32(__floats2half2_rn(p0, p1));
             }
             tmem_store16(s_at + 16 * ch, p);
           }
-          l += l2;
+          const float2 sum = unpair(add2(sums[0], sums[1]));
+          l += sum.x + sum.y;
           tc_wait_st();
           tc_fence_before();
           arrive(bars + 8 * (kWeights + x));
@@ -386,6 +422,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
     }
     if (threadIdx.x == 0) a.join_how[piece] = (uint8_t)how;
   } else if (warp < kMmaWarp) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kDeqRegs));
     // --------------------------------------------------------- dequantising
     const int dw = warp - kSoftWarps, g = lane >> 2, t = lane & 3;
     constexpr int kWords = D / 32, kGroupWords = kWords / NG;
@@ -537,58 +574,62 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
       }
     }
   } else {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kMmaRegs));
     // --------------------------------------------------------- the products
+    more = more && warp == kMmaWarp;
     constexpr uint32_t kShapeS = product_shape(kTok), kShapeO = product_shape(D);
+    const uint32_t tm = uniform(tmem), at = uniform(base);
     uint32_t weights_parity[2] = {0, 0}, query_parity[2] = {0, 0};
     int no = 0;  // tile of the piece
+    auto scores = [&](int x, int half) {
+      tc_fence_after();
+      if (elected()) {
+        const uint32_t qa = operand_low(at + F::kQ + x * F::kOperand), kb = operand_low(at + F::kK + half * F::kOperand);
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k) {
+          const uint32_t off = ((k / 4) * 16384 + (k % 4) * 32) >> 4;
+          if (k == 0) product_ss<false>(tm + x * kTok, qa, kb, kShapeS);
+          else product_ss<true>(tm + x * kTok, qa + off, kb + off, kShapeS);
+        }
+        tc_commit(bars + 8 * (kScores + x));
+      }
+      __syncwarp();
+    };
+    auto values = [&](int x, int half, bool add, bool release) {
+      tc_fence_after();
+      if (elected()) {
+        const uint32_t vb = operand_low(at + F::kV + half * F::kOperand);
+#pragma unroll
+        for (int k = 0; k < kTok / 16; ++k)
+          product_ts(tm + 2 * kTok + x * D, tm + x * kTok + 8 * k, vb + (((k / 4) * (D * 128) + (k % 4) * 32) >> 4),
+                     kShapeO, k > 0 ? 1u : (uint32_t)add);
+        if (release) tc_commit(bars + 8 * (kEmpty + half));
+      }
+      __syncwarp();
+    };
     for (; more && fine; more = next_in_piece<L>(a, c.kv_heads, most, units, w)) {
-      const int n = w.t1 - w.t0;
-      const bool two = w.it.qn * a.ratio - w.it.rt * L::kRows > kTileRows;
-      auto scores = [&](int x, int half) {
-        if (lane == 0) {
-          tc_fence_after();
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            const uint32_t off = (k / 4) * 16384 + (k % 4) * 32;
-            product_ss(tmem + x * kTok, operand(base + F::kQ + x * F::kOperand + off),
-                       operand(base + F::kK + half * F::kOperand + off), kShapeS, k > 0);
-          }
-          tc_commit(bars + 8 * (kScores + x));
-        }
-        __syncwarp();
-      };
-      auto values = [&](int x, int half, bool add) {
-        if (lane == 0) {
-          tc_fence_after();
-#pragma unroll
-          for (int k = 0; k < kTok / 16; ++k)
-            product_ts(tmem + 2 * kTok + x * D, tmem + x * kTok + 8 * k,
-                       operand(base + F::kV + half * F::kOperand + (k / 4) * (D * 128) + (k % 4) * 32), kShapeO,
-                       add || k > 0);
-        }
-        __syncwarp();
-      };
+      const int n = (int)uniform(w.t1 - w.t0);
+      const int tiles = uniform(w.it.qn * a.ratio - w.it.rt * L::kRows > kTileRows) ? 2 : 1;  // of rows
       fine = fine && warp_wait(bars + 8 * (kFull + (no & 1)), no >> 1 & 1);
-      for (int x = 0; x < (two ? 2 : 1) && fine; ++x) {
+      for (int x = 0; x < tiles && fine; ++x) {
         fine = warp_wait(bars + 8 * (kQuery + x), query_parity[x]);
         query_parity[x] ^= 1;
         if (fine) scores(x, no & 1);
       }
       for (int j = 0; j < n && fine; ++j, ++no) {
         const int half = no & 1, next = (no + 1) & 1;
-        for (int x = 0; x < (two ? 2 : 1) && fine; ++x) {
+        for (int x = 0; x < tiles && fine; ++x) {
           fine = warp_wait(bars + 8 * (kWeights + x), weights_parity[x]);
           weights_parity[x] ^= 1;
           if (!fine) break;
-          values(x, half, j > 0);
-          if (x == (two ? 1 : 0) && lane == 0) tc_commit(bars + 8 * (kEmpty + half));
+          values(x, half, j > 0, x == tiles - 1);
           if (j + 1 < n) {
             if (x == 0) fine = warp_wait(bars + 8 * (kFull + next), (no + 1) >> 1 & 1);
             if (fine) scores(x, next);
-          } else if (lane == 0) {
-            tc_commit(bars + 8 * (kScores + x));  // O is complete
+          } else {
+            if (elected()) tc_commit(bars + 8 * (kScores + x));  // O is complete
+            __syncwarp();
           }
-          __syncwarp();
         }
       }
     }
