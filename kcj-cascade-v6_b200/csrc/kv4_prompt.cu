@@ -185,7 +185,17 @@ CB_D __half2 code_high(uint32_t w) {
 }
 
 // Barriers, 8 bytes each.
-enum { kFull = 0, kEmpty = 2, kScores = 4, kWeights = 6, kQuery = 8, kRawBars = 10, kBarCount = kRawBars + kDeqWarps * kRaw };
+enum {
+  kFullK = 0,
+  kFullV = 2,
+  kEmptyK = 4,
+  kEmptyV = 6,
+  kScores = 8,
+  kWeights = 10,
+  kQuery = 12,
+  kRawBars = 14,
+  kBarCount = kRawBars + kDeqWarps * kRaw
+};
 
 template <int D, int NG>
 __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const Kv4View c, const AttendArgs a) {
@@ -209,8 +219,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
   if (warp == kMmaWarp) {
     if (lane == 0) {
       for (int i = 0; i < 2; ++i) {
-        bar_init(bars + 8 * (kFull + i), kDeqWarps * 32);
-        bar_init(bars + 8 * (kEmpty + i), 1);
+        bar_init(bars + 8 * (kFullK + i), kDeqWarps * 32);
+        bar_init(bars + 8 * (kFullV + i), kDeqWarps * 32);
+        bar_init(bars + 8 * (kEmptyK + i), 1);
+        bar_init(bars + 8 * (kEmptyV + i), 1);
         bar_init(bars + 8 * (kScores + i), 1);
         bar_init(bars + 8 * (kWeights + i), kTileRows);
         bar_init(bars + 8 * (kQuery + i), kTileRows);
@@ -484,18 +496,34 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
       const Item &it = w.it;
       const int last = min((it.rt + 1) * L::kRows, it.qn * a.ratio) - 1, sees_most = row_limit(a, it, last);
       for (int tl = w.t0; tl < w.t1 && fine; ++tl, ++no) {
-        const int half = no & 1;
-        fine = warp_wait(bars + 8 * (kEmpty + half), (no >> 1 & 1) ^ 1);
+        // K of both cache tiles, then V: a buffer of K is free again after the
+        // scores, one of V only after the second row tile's values.
+        const int half = no & 1, next = stage + 1 == kRaw ? 0 : stage + 1;
+        fine = warp_wait(bars + 8 * (kEmptyK + half), (no >> 1 & 1) ^ 1);
+        fine = fine && warp_wait(raw_bars + 8 * stage, raw_parity >> stage & 1);
+        fine = fine && warp_wait(raw_bars + 8 * next, raw_parity >> next & 1);
+        if (!fine) break;
+        raw_parity ^= 1u << stage | 1u << next;
+        const uint32_t there = (ok >> stage & 1) | (ok >> next & 1) << 1;
         uint8_t *k_to = smem + F::kK + half * F::kOperand, *v_to = smem + F::kV + half * F::kOperand;
-        uint32_t there = 0, bad = 0;
-#pragma unroll 1
-        for (int ct = 0; ct < 2 && fine; ++ct) {
-          fine = warp_wait(raw_bars + 8 * stage, raw_parity >> stage & 1);
-          raw_parity ^= 1u << stage;
-          const uint32_t here = ok >> stage & 1;
-          there |= here << ct;
-          const uint8_t *buf = ring + stage * F::kTile;
-          // ---- K: rows g and g + 8, 8 dims of 32 a word
+        const int tok0 = tl * kTok + dw * 32;
+        {  // lane: a token
+          const uint32_t *vp = reinterpret_cast<const uint32_t *>(ring + (lane < 16 ? stage : next) * F::kTile + 16 * D +
+                                                                  64 * NG) + (lane & 15) * NG;
+          bool bad = false;  // an exponent of all ones in a scale or an offset
+#pragma unroll
+          for (int gi = 0; gi < NG; ++gi) bad |= (vp[gi] & 0x7c00) == 0x7c00 || (vp[gi] >> 16 & 0x7c00) == 0x7c00;
+          bad = bad && tok0 + lane < sees_most && (there >> (lane >> 4) & 1);
+          const uint32_t votes = __ballot_sync(0xffffffffu, bad);
+          if (lane == 0) {
+            flags[no & 3].bad[dw] = votes;
+            reinterpret_cast<uint8_t *>(&flags[no & 3].there)[dw] = (uint8_t)there;
+          }
+        }
+#pragma unroll
+        for (int ct = 0; ct < 2; ++ct) {
+          const uint8_t *buf = ring + (ct ? next : stage) * F::kTile;
+          // rows g and g + 8, 8 dims of 32 a word
           uint32_t kw[2][kWords], kp[2][NG];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -523,25 +551,27 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
               *reinterpret_cast<uint4 *>(k_to + (i >> 1) * 16384 + row * 128 + ((((i & 1) * 4 + t) ^ (row & 7)) << 4)) = y;
             }
           }
-          // ---- V: token pairs 8 h + 2t, 4 dims a word
-          const int tok0 = tl * kTok + dw * 32 + ct * 16;
+        }
+        fence_async();
+        arrive(bars + 8 * (kFullK + half));
+        fine = warp_wait(bars + 8 * (kEmptyV + half), (no >> 1 & 1) ^ 1);
+        if (!fine) break;
+#pragma unroll
+        for (int ct = 0; ct < 2; ++ct) {
+          const uint8_t *buf = ring + (ct ? next : stage) * F::kTile;
+          // token pairs 8 h + 2t, 4 dims a word
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             uint32_t vw[kWords], vp[2 * NG];
             load_words<kWords>(buf + 8 * D + (h * 32 + lane) * 4 * kWords, vw);
             load_words<2 * NG>(buf + 16 * D + 64 * NG + (8 * h + 2 * t) * NG * 4, vp);
-            const int tok = tok0 + 8 * h + 2 * t;
-            const bool on0 = here && tok < sees_most, on1 = here && tok + 1 < sees_most;
-            bool bad0 = false, bad1 = false;
+            const int tok = tok0 + ct * 16 + 8 * h + 2 * t;
+            const bool on0 = (there >> ct & 1) && tok < sees_most, on1 = (there >> ct & 1) && tok + 1 < sees_most;
 #pragma unroll
             for (int gi = 0; gi < NG; ++gi) {
-              uint32_t p0 = on0 ? vp[gi] : 0, p1 = on1 ? vp[NG + gi] : 0;
-              // an exponent of all ones in the scale or the offset
-              const bool b0 = (p0 & 0x7c00) == 0x7c00 || (p0 >> 16 & 0x7c00) == 0x7c00;
-              const bool b1 = (p1 & 0x7c00) == 0x7c00 || (p1 >> 16 & 0x7c00) == 0x7c00;
-              bad0 |= b0, bad1 |= b1;
-              if (b0) p0 = 0;
-              if (b1) p1 = 0;
+              uint32_t p0 = vp[gi], p1 = vp[NG + gi];
+              if (!on0 || (p0 & 0x7c00) == 0x7c00 || (p0 >> 16 & 0x7c00) == 0x7c00) p0 = 0;
+              if (!on1 || (p1 & 0x7c00) == 0x7c00 || (p1 >> 16 & 0x7c00) == 0x7c00) p1 = 0;
               const __half2 sc = as_half2(__byte_perm(p0, p1, 0x5410)), of = as_half2(__byte_perm(p0, p1, 0x7632));
 #pragma unroll
               for (int j = gi * kGroupWords; j < (gi + 1) * kGroupWords; ++j) {
@@ -557,20 +587,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
                                                 ((chunk ^ g) << 4) + 4 * t) = y[k];
               }
             }
-            if (bad0) bad |= 1u << (ct * 16 + 8 * h + 2 * t);
-            if (bad1) bad |= 2u << (ct * 16 + 8 * h + 2 * t);
           }
           __syncwarp();
-          ahead_issue(stage);
-          stage = stage + 1 == kRaw ? 0 : stage + 1;
-        }
-        bad = __reduce_or_sync(0xffffffffu, bad);
-        if (lane == 0) {
-          flags[no & 3].bad[dw] = bad;
-          reinterpret_cast<uint8_t *>(&flags[no & 3].there)[dw] = (uint8_t)there;
+          ahead_issue(ct ? next : stage);
         }
         fence_async();
-        arrive(bars + 8 * (kFull + half));
+        arrive(bars + 8 * (kFullV + half));
+        stage = next + 1 == kRaw ? 0 : next + 1;
       }
     }
   } else {
@@ -581,7 +604,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
     const uint32_t tm = uniform(tmem), at = uniform(base);
     uint32_t weights_parity[2] = {0, 0}, query_parity[2] = {0, 0};
     int no = 0;  // tile of the piece
-    auto scores = [&](int x, int half) {
+    auto scores = [&](int x, int half, bool release) {
       tc_fence_after();
       if (elected()) {
         const uint32_t qa = operand_low(at + F::kQ + x * F::kOperand), kb = operand_low(at + F::kK + half * F::kOperand);
@@ -592,6 +615,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
           else product_ss<true>(tm + x * kTok, qa + off, kb + off, kShapeS);
         }
         tc_commit(bars + 8 * (kScores + x));
+        if (release) tc_commit(bars + 8 * (kEmptyK + half));
       }
       __syncwarp();
     };
@@ -603,29 +627,30 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
         for (int k = 0; k < kTok / 16; ++k)
           product_ts(tm + 2 * kTok + x * D, tm + x * kTok + 8 * k, vb + (((k / 4) * (D * 128) + (k % 4) * 32) >> 4),
                      kShapeO, k > 0 ? 1u : (uint32_t)add);
-        if (release) tc_commit(bars + 8 * (kEmpty + half));
+        if (release) tc_commit(bars + 8 * (kEmptyV + half));
       }
       __syncwarp();
     };
     for (; more && fine; more = next_in_piece<L>(a, c.kv_heads, most, units, w)) {
       const int n = (int)uniform(w.t1 - w.t0);
       const int tiles = uniform(w.it.qn * a.ratio - w.it.rt * L::kRows > kTileRows) ? 2 : 1;  // of rows
-      fine = fine && warp_wait(bars + 8 * (kFull + (no & 1)), no >> 1 & 1);
+      fine = fine && warp_wait(bars + 8 * (kFullK + (no & 1)), no >> 1 & 1);
       for (int x = 0; x < tiles && fine; ++x) {
         fine = warp_wait(bars + 8 * (kQuery + x), query_parity[x]);
         query_parity[x] ^= 1;
-        if (fine) scores(x, no & 1);
+        if (fine) scores(x, no & 1, x == tiles - 1);
       }
       for (int j = 0; j < n && fine; ++j, ++no) {
         const int half = no & 1, next = (no + 1) & 1;
         for (int x = 0; x < tiles && fine; ++x) {
           fine = warp_wait(bars + 8 * (kWeights + x), weights_parity[x]);
           weights_parity[x] ^= 1;
+          if (x == 0) fine = fine && warp_wait(bars + 8 * (kFullV + half), no >> 1 & 1);
           if (!fine) break;
           values(x, half, j > 0, x == tiles - 1);
           if (j + 1 < n) {
-            if (x == 0) fine = warp_wait(bars + 8 * (kFull + next), (no + 1) >> 1 & 1);
-            if (fine) scores(x, next);
+            if (x == 0) fine = warp_wait(bars + 8 * (kFullK + next), (no + 1) >> 1 & 1);
+            if (fine) scores(x, next, x == tiles - 1);
           } else {
             if (elected()) tc_commit(bars + 8 * (kScores + x));  // O is complete
             __syncwarp();
