@@ -19,7 +19,7 @@
 // product for a score, where exact codes would need one for every group and two
 // multiplications for every score), P, and the output; q is exact, as in
 // kv4_attend.cu. A V that is NaN or infinite is zero as an operand, or rows that
-// do not see its token would be hurt; rows that do see it become NaN.
+// do not see its token would be hurt; rows that do see it (or such a K) become NaN.
 #include "kv4_attend.cuh"
 
 namespace cb {
@@ -43,7 +43,7 @@ struct PromptLine {
 };
 
 struct TileFlags {  // of 128 tokens, written by the dequantising warps
-  uint32_t bad[4];  // a bit for each token whose V is not finite
+  uint32_t bad[4];  // a bit for each token whose K or V is not finite
   uint32_t there;   // two bits in each warp's byte: its cache tiles are there
   uint32_t pad[3];
 };
@@ -146,6 +146,12 @@ CB_D void tmem_store16(uint32_t addr, const uint32_t *r) {
 CB_D void fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 CB_D void arrive(uint32_t bar) { asm volatile("mbarrier.arrive.shared.b64 _, [%0];" ::"r"(bar) : "memory"); }
 
+// A warp's arrival, after what all its lanes have done.
+CB_D void warp_arrive(uint32_t bar) {
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0) arrive(bar);
+}
+
 // A wait of a whole warp, which goes one way for all of it.
 CB_D bool warp_wait(uint32_t bar, uint32_t parity) { return __all_sync(0xffffffffu, bar_wait(bar, parity)); }
 
@@ -168,6 +174,12 @@ CB_D uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
 CB_D uint64_t add2(uint64_t a, uint64_t b) {
   uint64_t v;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v) : "l"(a), "l"(b));
+  return v;
+}
+
+CB_D float max3(float x, float y, float z) {
+  float v;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(v) : "f"(x), "f"(y), "f"(z));
   return v;
 }
 
@@ -219,13 +231,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
   if (warp == kMmaWarp) {
     if (lane == 0) {
       for (int i = 0; i < 2; ++i) {
-        bar_init(bars + 8 * (kFullK + i), kDeqWarps * 32);
-        bar_init(bars + 8 * (kFullV + i), kDeqWarps * 32);
+        bar_init(bars + 8 * (kFullK + i), kDeqWarps);
+        bar_init(bars + 8 * (kFullV + i), kDeqWarps);
         bar_init(bars + 8 * (kEmptyK + i), 1);
         bar_init(bars + 8 * (kEmptyV + i), 1);
         bar_init(bars + 8 * (kScores + i), 1);
-        bar_init(bars + 8 * (kWeights + i), kTileRows);
-        bar_init(bars + 8 * (kQuery + i), kTileRows);
+        bar_init(bars + 8 * (kWeights + i), kTileRows / 32);
+        bar_init(bars + 8 * (kQuery + i), kTileRows / 32);
       }
       for (int i = 0; i < kDeqWarps * kRaw; ++i) bar_init(bars + 8 * (kRawBars + i), 1);
       asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -306,7 +318,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
                                      (((i & 7) ^ (r & 7)) << 4)) = make_uint4(z[0], z[1], z[2], z[3]);
         }
         fence_async();
-        arrive(bars + 8 * (kQuery + x));
+        warp_arrive(bars + 8 * (kQuery + x));
 
         const int limit = row_limit(a, it, min(row, total - 1));
         float l = 0.0f, over = -INFINITY, sub = 0.0f;
@@ -333,7 +345,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
 #pragma unroll
           for (int k = 0; k < kTok; k += 8)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) tops[i] = fmaxf(tops[i], fmaxf(v[k + 2 * i], v[k + 2 * i + 1]));
+            for (int i = 0; i < 4; ++i) tops[i] = max3(tops[i], v[k + 2 * i], v[k + 2 * i + 1]);
           const float top2 = fmaxf(tops[0], tops[1]), top3 = fmaxf(tops[2], tops[3]);
           const float m = fmaxf(top2, top3) * to_log2;
           float f = 1.0f;
@@ -381,7 +393,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
           l += sum.x + sum.y;
           tc_wait_st();
           tc_fence_before();
-          arrive(bars + 8 * (kWeights + x));
+          warp_arrive(bars + 8 * (kWeights + x));
         }
         // ---- out, or a part of it
         if (fine) {
@@ -508,11 +520,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
         uint8_t *k_to = smem + F::kK + half * F::kOperand, *v_to = smem + F::kV + half * F::kOperand;
         const int tok0 = tl * kTok + dw * 32;
         {  // lane: a token
-          const uint32_t *vp = reinterpret_cast<const uint32_t *>(ring + (lane < 16 ? stage : next) * F::kTile + 16 * D +
-                                                                  64 * NG) + (lane & 15) * NG;
+          const uint32_t *kp = reinterpret_cast<const uint32_t *>(ring + (lane < 16 ? stage : next) * F::kTile + 16 * D) +
+                               (lane & 15) * NG;
           bool bad = false;  // an exponent of all ones in a scale or an offset
 #pragma unroll
-          for (int gi = 0; gi < NG; ++gi) bad |= (vp[gi] & 0x7c00) == 0x7c00 || (vp[gi] >> 16 & 0x7c00) == 0x7c00;
+          for (int gi = 0; gi < NG; ++gi) {
+            const uint32_t pk = kp[gi], pv = kp[16 * NG + gi];
+            bad |= (pk & 0x7c00) == 0x7c00 || (pk >> 16 & 0x7c00) == 0x7c00;
+            bad |= (pv & 0x7c00) == 0x7c00 || (pv >> 16 & 0x7c00) == 0x7c00;
+          }
           bad = bad && tok0 + lane < sees_most && (there >> (lane >> 4) & 1);
           const uint32_t votes = __ballot_sync(0xffffffffu, bad);
           if (lane == 0) {
@@ -553,7 +569,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
           }
         }
         fence_async();
-        arrive(bars + 8 * (kFullK + half));
+        warp_arrive(bars + 8 * (kFullK + half));
         fine = warp_wait(bars + 8 * (kEmptyV + half), (no >> 1 & 1) ^ 1);
         if (!fine) break;
 #pragma unroll
@@ -592,7 +608,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
           ahead_issue(ct ? next : stage);
         }
         fence_async();
-        arrive(bars + 8 * (kFullV + half));
+        warp_arrive(bars + 8 * (kFullV + half));
         stage = next + 1 == kRaw ? 0 : next + 1;
       }
     }
