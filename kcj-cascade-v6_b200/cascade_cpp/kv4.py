@@ -60,17 +60,27 @@ def _device(device) -> "torch.device":
     return torch.device("cuda", torch.cuda.current_device()) if d.index is None else d
 
 
+# torch.cuda.current_stream(device).cuda_stream without the two objects it makes
+_raw_stream = getattr(getattr(torch, "_C", None), "_cuda_getCurrentRawStream", None)
+
+
 def _stream(device):
+    if _raw_stream is not None:
+        return _raw_stream(device.index)
     return torch.cuda.current_stream(device).cuda_stream
+
+
+def _on(t, name: str, device):
+    if not isinstance(t, torch.Tensor) or t.get_device() != device.index:  # -1 for the host
+        raise TypeError(f"{name} must be a tensor on {device}")
 
 
 def _vector(t, name: str, dtype, device, n=None):
     """Address of a contiguous 1-D tensor of the device."""
-    if not isinstance(t, torch.Tensor) or t.device != device:
-        raise TypeError(f"{name} must be a tensor on {device}")
-    if t.dtype != dtype:
+    _on(t, name, device)
+    if t.dtype is not dtype:
         raise TypeError(f"{name} must be {dtype}")
-    if t.dim() != 1 or (n is not None and t.shape[0] != n) or not t.is_contiguous():
+    if t.dim() != 1 or (n is not None and t.numel() != n) or not t.is_contiguous():
         raise ValueError(f"{name} must be a contiguous vector" + ("" if n is None else f" of {n}"))
     return t.data_ptr()
 
@@ -127,6 +137,7 @@ class KV4Cache(KVPageConnector):
         self.layers, self.kv_heads, self.head_dim = int(layers), int(heads), int(head_dim)
         self.page_size, self.group = int(page_size), int(group)
         self.errors = torch.zeros(1, dtype=torch.int32, device=self.device)
+        self._work: dict = {}
         stride = self.stride if self.num_pages > 1 else max(self.stride, self.page_bytes)
         self._form = L.cb_kv4_cache(self.base, stride, self.errors.data_ptr(), self.num_pages, self.layers,
                                     self.kv_heads, self.head_dim, self.page_size, self.group, self.device.index, 0)
@@ -146,8 +157,7 @@ class KV4Cache(KVPageConnector):
     # ------------------------------------------------------------ operators
 
     def _values(self, t, name: str):
-        if not isinstance(t, torch.Tensor) or t.device != self.device:
-            raise TypeError(f"{name} must be a tensor on {self.device}")
+        _on(t, name, self.device)
         if t.dim() != 3 or t.shape[1] != self.kv_heads or t.shape[2] != self.head_dim or (
                 t.stride(2) != 1 and t.numel()):
             raise ValueError(f"{name} must be [tokens, {self.kv_heads}, {self.head_dim}] with contiguous heads")
@@ -199,8 +209,7 @@ class KV4Cache(KVPageConnector):
         were in ``out``. With ``return_lse`` also the log-sum-exp of each row's
         scores, ``[total_q, q_heads]`` fp32. There is no backward pass."""
         dev, d = self.device, self.head_dim
-        if not isinstance(q, torch.Tensor) or q.device != dev:
-            raise TypeError(f"q must be a tensor on {dev}")
+        _on(q, "q", dev)
         if q.dim() != 3 or q.shape[2] != d or (q.stride(2) != 1 and q.numel()):
             raise ValueError(f"q must be [rows, q_heads, {d}] with contiguous heads")
         if q.requires_grad and torch.is_grad_enabled():
@@ -209,8 +218,9 @@ class KV4Cache(KVPageConnector):
         if heads == 0 or heads % self.kv_heads:
             raise ValueError(f"q_heads must be a multiple of {self.kv_heads}")
         code = _dtype_code(q.dtype)
-        if not isinstance(block_table, torch.Tensor) or block_table.device != dev or block_table.dtype != torch.int32:
-            raise TypeError(f"block_table must be an int32 tensor on {dev}")
+        _on(block_table, "block_table", dev)
+        if block_table.dtype is not torch.int32:
+            raise TypeError("block_table must be torch.int32")
         if block_table.dim() != 2 or block_table.shape[1] == 0 or (
                 block_table.stride(1) != 1 and block_table.shape[1] > 1):
             raise ValueError("block_table must be [requests, columns] with contiguous rows")
@@ -233,10 +243,11 @@ class KV4Cache(KVPageConnector):
             d ** -0.5 if scale is None else scale, layer, code, n, columns, rows, heads,
             (1 if start is None else rows) if max_q is None else max_q, causal, 0)
         lib = _native_lib()
-        need = lib.cb_kv4_attend_workspace(self._form, a)
-        if need:
-            work = torch.empty(need, dtype=torch.uint8, device=dev)
-            a.workspace, a.workspace_bytes = work.data_ptr(), need
+        need = self._work.get((heads, a.max_q))  # the sizes that decide it
+        if need is None:
+            need = self._work[heads, a.max_q] = lib.cb_kv4_attend_workspace(self._form, a)
+        work = torch.empty(need, dtype=torch.uint8, device=dev)
+        a.workspace, a.workspace_bytes = work.data_ptr(), need
         _check(lib.cb_kv4_attend(self._form, a, _stream(dev)))
         return out if lse is None else (out, lse)
 

@@ -66,8 +66,13 @@ namespace {
 // its share of the tokens; the cluster's barrier stands between reading the old
 // state and writing the new one, so the state may be updated in place with one
 // launch and no counters in memory.
+//
+// A warp takes 8 x 32 tokens at a time (32 where there are few): each lane's eight
+// rows are found first, then its eight page numbers are under way together; one at a
+// time, every token would wait for a search and a load.
 constexpr int kPlanThreads = 512;
-constexpr int kPlanCtas = 8;
+constexpr int kPlanCtas = 16;  // the largest cluster
+constexpr int kPlanRun = 8;
 
 // Exclusive prefix sum over the block; `total` is the block's sum.
 CB_D long long block_scan(long long x, long long *warp_sums, long long &total) {
@@ -108,11 +113,14 @@ CB_D void plan_barrier(int ctas) {
   else __syncthreads();
 }
 
+template <int RUN>
 __global__ void __launch_bounds__(kPlanThreads) kv4_plan_kernel(const cb_kv4_plan_args a, const int ctas) {
   __shared__ long long start[kPlanThreads + 1], base[kPlanThreads], warp_sums[kPlanThreads / 32];
   __shared__ int len_s[kPlanThreads], held_s[kPlanThreads];  // held_s: -1 for a refused row
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, lane = tid & 31;
+  const long long stride = (long long)ctas * kPlanThreads * RUN;  // of the cluster
   const int rank = ctas > 1 ? (int)cg::this_cluster().block_rank() : 0;
+  const long long mine = ((long long)rank * kPlanThreads + (tid & ~31)) * RUN + lane;
   const int ps = a.page_size;
   const long long most = (long long)a.columns * ps;
   long long count = min(max(*a.free_count, 0), a.num_pages);
@@ -138,12 +146,21 @@ __global__ void __launch_bounds__(kPlanThreads) kv4_plan_kernel(const cb_kv4_pla
       start[tid] = at;
       held_s[tid] = bor;
       __syncthreads();
-      for (long long e = (long long)rank * kPlanThreads + tid; e < total; e += (long long)ctas * kPlanThreads) {
-        const int i = find_row(start, kPlanThreads, e);
-        const int page = a.block_table[(r0 + i) * a.table_stride + held_s[i] + (e - start[i])];
-        const long long to = count + back + e;
-        if (to < a.num_pages) a.free[to] = page;
-        else kv4_error(a.errors, kErrBounds);  // more pages came back than there are
+      for (long long e0 = mine; e0 - lane < total; e0 += stride) {
+        int page[RUN];
+        int i = e0 < total ? find_row(start, kPlanThreads, e0) : 0;
+#pragma unroll
+        for (int u = 0; u < RUN; ++u) {
+          const long long e = e0 + 32 * u;
+          while (e < total && i + 1 < kPlanThreads && start[i + 1] <= e) ++i;
+          if (e < total) page[u] = a.block_table[(r0 + i) * a.table_stride + held_s[i] + (e - start[i])];
+        }
+#pragma unroll
+        for (int u = 0; u < RUN; ++u) {
+          const long long e = e0 + 32 * u, to = count + back + e;
+          if (e < total && to < a.num_pages) a.free[to] = page[u];
+          else if (e < total) kv4_error(a.errors, kErrBounds);  // more pages came back than there are
+        }
       }
       back += total;
       __syncthreads();
@@ -186,26 +203,40 @@ __global__ void __launch_bounds__(kPlanThreads) kv4_plan_kernel(const cb_kv4_pla
     }
     __syncthreads();
     const long long end = min(tokens + total, (long long)a.tokens);
-    for (long long n = tokens + (long long)rank * kPlanThreads + tid; n < end;
-         n += (long long)ctas * kPlanThreads) {
-      const int i = find_row(start, kPlanThreads, n);
-      const long long pos = len_s[i] + (n - start[i]);
-      long long slot = -1;
-      if (held_s[i] >= 0) {
-        const long long col = pos / ps;
-        int32_t *entry = a.block_table + (r0 + i) * a.table_stride + col;
-        int page;
-        if (col < held_s[i]) {
-          page = *entry;
-        } else {
-          page = a.free[count - 1 - (base[i] + col - held_s[i])];
-          if (pos == col * ps) *entry = page;  // the first token of a new page
+    for (long long n0 = tokens + mine; n0 - lane < end; n0 += stride) {
+      int page[RUN], pos[RUN], row[RUN];
+      int i = n0 < end ? find_row(start, kPlanThreads, n0) : 0;
+#pragma unroll
+      for (int u = 0; u < RUN; ++u) {
+        const long long n = n0 + 32 * u;
+        while (n < end && i + 1 < kPlanThreads && start[i + 1] <= n) ++i;
+        page[u] = -1, pos[u] = 0, row[u] = -1;
+        if (n < end) {
+          const long long p = len_s[i] + (n - start[i]);
+          pos[u] = (int)min(p, 0x7fffffffll);
+          if (held_s[i] >= 0) {
+            const int col = pos[u] / ps;
+            row[u] = i;
+            page[u] = col < held_s[i] ? a.block_table[(r0 + i) * a.table_stride + col]
+                                      : a.free[count - 1 - (base[i] + col - held_s[i])];
+          }
         }
-        if (page >= 0 && page < a.num_pages) slot = (long long)page * ps + (pos - col * ps);
-        else kv4_error(a.errors, kErrBounds);
       }
-      a.slots[n] = slot;
-      a.positions[n] = (int)min(pos, 0x7fffffffll);
+#pragma unroll
+      for (int u = 0; u < RUN; ++u) {
+        const long long n = n0 + 32 * u;
+        if (n >= end) break;
+        long long slot = -1;
+        if (row[u] >= 0) {
+          const int col = pos[u] / ps, in_page = pos[u] - col * ps;
+          if (in_page == 0 && col >= held_s[row[u]])  // the first token of a new page
+            a.block_table[(r0 + row[u]) * a.table_stride + col] = page[u];
+          if (page[u] >= 0 && page[u] < a.num_pages) slot = (long long)page[u] * ps + in_page;
+          else kv4_error(a.errors, kErrBounds);
+        }
+        a.slots[n] = slot;
+        a.positions[n] = pos[u];
+      }
     }
     tokens += total;
     needed += need_total;
@@ -234,12 +265,17 @@ __global__ void __launch_bounds__(kPlanThreads) kv4_plan_kernel(const cb_kv4_pla
 
 // ---------------------------------------------------------- append and read
 //
-// A thread holds 8 adjacent dimensions of one token's keys or values of one
-// head, so a row of D values is D/8 adjacent lanes: the group's minimum and
-// maximum are shuffles among group/8 of them, and the word of codes of K is
-// one lane's own. A 16-bit word of V collects a nibble from each of four
-// adjacent lanes (dims 8 apart), which they exchange by shuffles.
+// A warp takes 8 tokens of the call, wherever their slots are, and K or V of one
+// head. In registers a lane (g, t) has the dims 32 i + 8 t .. + 7 of token g: 64
+// contiguous bytes of a 16-bit row for every four lanes and i. For K that
+// is the order of the words in a page: a token's minimum and maximum are shuffles
+// among four lanes, and its row of codes is 16 bytes a lane. For V the lanes
+// exchange: four lanes collect the nibbles of dims 8 apart, then two rows their
+// halves of a word. Bound by HBM: 4 D bytes of values and 1 - 1.25 D of codes for
+// a token and head.
+constexpr int kTokenThreads = 128, kTokensWarp = 8;
 
+// 8 values; `vec`: on a 16-byte boundary.
 template <typename T>
 CB_D void load8(const T *p, bool vec, float *x) {
   if (vec) {
@@ -258,165 +294,271 @@ CB_D void load8(const T *p, bool vec, float *x) {
   }
 }
 
+template <typename T>
+CB_D void store8(T *p, bool vec, const float *x) {
+  alignas(16) T y[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = kv4_round<T>(x[i]);
+  if (vec) {
+#pragma unroll
+    for (int w = 0; w < (int)sizeof(T) / 2; ++w)
+      reinterpret_cast<uint4 *>(p)[w] = reinterpret_cast<const uint4 *>(y)[w];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) p[i] = y[i];
+  }
+}
+
 struct TokenStrides {
   int64_t k_token, k_head, v_token, v_head;
 };
 
-constexpr int kTokenThreads = 256;
+// Where a token of the call lives: its tile (of the head) and place, or no tile.
+struct Spot {
+  uint8_t *tile;
+  int tok;
+};
+
+// The spots of the warp's 8 tokens, one in each of lanes 0 .. 7.
+CB_D Spot load_spot(const Kv4View &c, const int64_t *slots, int64_t n, int64_t first, int head, int tile_bytes) {
+  const int lane = threadIdx.x & 31;
+  Spot s = {nullptr, 0};
+  if (lane < kTokensWarp && first + lane < n) {
+    const int64_t slot = __ldg(slots + first + lane);
+    const int64_t page = slot >> c.page_log2;
+    if (slot >= 0 && page < c.num_pages) {
+      const int in_page = (int)(slot & (c.page_size - 1));
+      s.tok = in_page % kKv4Tile;
+      s.tile = c.base + page * c.page_stride + head * c.head_bytes + (uint64_t)(in_page / kKv4Tile) * tile_bytes;
+    } else if (slot >= 0) {
+      kv4_error(c.errors, kErrBounds);
+    }
+  }
+  return s;
+}
+
+CB_D Spot spot_of(const Spot &s, int token) {
+  Spot r;
+  r.tile = reinterpret_cast<uint8_t *>(__shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(s.tile), token));
+  r.tok = __shfl_sync(0xffffffffu, s.tok, token);
+  return r;
+}
+
+template <int N>
+CB_D void load_words4(const void *p, uint32_t *w) {
+  if constexpr (N == 2) {
+    const uint2 v = *static_cast<const uint2 *>(p);
+    w[0] = v.x, w[1] = v.y;
+  } else {
+    const uint4 v = *static_cast<const uint4 *>(p);
+    w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+  }
+}
+template <int N>
+CB_D void store_words4(void *p, const uint32_t *w) {
+  if constexpr (N == 2) *static_cast<uint2 *>(p) = make_uint2(w[0], w[1]);
+  else *static_cast<uint4 *>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+}
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kTokenThreads)
     kv4_append_kernel(const Kv4View c, const int group, const T *__restrict__ k, const T *__restrict__ v,
                       const TokenStrides st, const bool vec, const int64_t *__restrict__ slots, const int n) {
-  constexpr int kLanes = D / 8, kWords = (D < 128 ? D : 128) / 32;
-  const int64_t rows = (int64_t)n * 2 * c.kv_heads;
-  const int64_t id = (int64_t)blockIdx.x * kTokenThreads + threadIdx.x;
-  int64_t row = id / kLanes;
-  const int lane = (int)(id % kLanes);
-  const bool there = row < rows;
-  if (!there) row = rows - 1;  // every lane of a warp takes part in the shuffles
-  const int head = (int)(row % c.kv_heads);
-  const int64_t tk = row / c.kv_heads;
-  const bool is_v = tk & 1;
-  const int64_t token = tk >> 1;
-
-  float x[8];
-  const T *src = is_v ? v + token * st.v_token + head * st.v_head : k + token * st.k_token + head * st.k_head;
-  load8(src + lane * 8, vec, x);
-  // fmin/fmax drop a NaN; a sum that is NaN keeps it (the values are finite otherwise)
-  float lo = INFINITY, hi = -INFINITY, nan = 0.0f;
+  constexpr int kSlabs = D > 128 ? 2 : 1, kWpr = D / kSlabs / 32, kWords = D / 32;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, ng = D / group;
+  const int64_t id = (int64_t)blockIdx.x * (kTokenThreads / 32) + (threadIdx.x >> 5);
+  const int head = (int)(id % c.kv_heads);
+  const bool is_v = id / c.kv_heads & 1;
+  const int64_t first = id / c.kv_heads / 2 * kTokensWarp;
+  if (first >= n) return;
+  const Spot mine = load_spot(c, slots, n, first, head, kv4_tile_bytes(D, group));
+  uint32_t words[kWords];  // codes of token g: dims 8 t + e of block i in nibble e
+  {
+    const Spot to = spot_of(mine, g);
+    const int64_t row = first + (first + g < n ? g : 0);
+    const T *src = (is_v ? v + row * st.v_token + head * st.v_head : k + row * st.k_token + head * st.k_head) + 8 * t;
+    float x[kWords][8], lo[kWords], hi[kWords], nan[kWords];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if (x[i] != x[i]) nan = x[i];
-    x[i] = fminf(fmaxf(x[i], -kKv4Most), kKv4Most);
-    lo = fminf(lo, x[i]);
-    hi = fmaxf(hi, x[i]);
-  }
-  for (int o = 1; o < group / 8; o <<= 1) {
-    lo = fminf(lo, __shfl_xor_sync(0xffffffffu, lo, o));
-    hi = fmaxf(hi, __shfl_xor_sync(0xffffffffu, hi, o));
-    nan += __shfl_xor_sync(0xffffffffu, nan, o);
-  }
-  const __half scale_h = __float2half_rn(__fadd_rn(__fdiv_rn(__fsub_rn(hi, lo), 15.0f), nan));
-  const float s = __half2float(scale_h);
-  const __half offset_h = __float2half_rn(__fadd_rn(lo, __fmul_rn(8.0f, s)));
-  const float o = __half2float(offset_h);
-  const float step = s > 0.0f ? __fdiv_rn(1.0f, s) : 0.0f;
-  uint32_t code[8];
+    for (int i = 0; i < kWords; ++i) load8(src + 32 * i, vec, x[i]);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float t = s > 0.0f ? rintf(__fmul_rn(__fsub_rn(x[i], o), step)) : 0.0f;
-    code[i] = (uint32_t)((int)fminf(fmaxf(t, -8.0f), 7.0f) + 8);
-  }
-
-  const int64_t slot = there ? __ldg(slots + token) : -1;
-  const int64_t page = slot >> c.page_log2;
-  const bool ok = slot >= 0 && page < c.num_pages;
-  if (slot >= 0 && !ok) kv4_error(c.errors, kErrBounds);
-  const int in_page = (int)(slot & (c.page_size - 1)), tok = in_page % kKv4Tile;
-  const int ng = D / group;
-  uint8_t *tile = c.base + (ok ? page : 0) * c.page_stride + head * c.head_bytes +
-                  (uint64_t)(in_page / kKv4Tile) * kv4_tile_bytes(D, group);
-  const int slab = lane / (kWords * 4), i = lane % (kWords * 4) / 4, t = lane % 4;
-  uint32_t word = 0;
-  if (!is_v) {
+    for (int i = 0; i < kWords; ++i) {
+      // fmin and fmax drop a NaN: it is carried beside them
+      lo[i] = INFINITY, hi[i] = -INFINITY, nan[i] = 0.0f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) word |= code[e] << (4 * ((e & 1) * 4 + e / 2));
+      for (int e = 0; e < 8; ++e) {
+        if (x[i][e] != x[i][e]) nan[i] = x[i][e];
+        x[i][e] = fminf(fmaxf(x[i][e], -kKv4Most), kKv4Most);
+        lo[i] = fminf(lo[i], x[i][e]);
+        hi[i] = fmaxf(hi[i], x[i][e]);
+      }
+    }
+#pragma unroll
+    for (int span = 1; span < kWords; span *= 2) {
+      if (group <= 32 * span) break;
+#pragma unroll
+      for (int i = 0; i < kWords; i += 2 * span) {
+        lo[i] = fminf(lo[i], lo[i + span]), hi[i] = fmaxf(hi[i], hi[i + span]), nan[i] += nan[i + span];
+      }
+    }
+    const int step_words = group / 32;
+    float off = 0.0f, inv = 0.0f;
+    bool any = false;
+    __half scale_h = __float2half_rn(0.0f), offset_h = scale_h;
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) {
+      if (i % step_words == 0) {  // a group begins: its parameters
+#pragma unroll
+        for (int o = 1; o < 4; o <<= 1) {
+          lo[i] = fminf(lo[i], __shfl_xor_sync(0xffffffffu, lo[i], o));
+          hi[i] = fmaxf(hi[i], __shfl_xor_sync(0xffffffffu, hi[i], o));
+          nan[i] += __shfl_xor_sync(0xffffffffu, nan[i], o);
+        }
+        scale_h = __float2half_rn(__fadd_rn(__fdiv_rn(__fsub_rn(hi[i], lo[i]), 15.0f), nan[i]));
+        const float s = __half2float(scale_h);
+        offset_h = __float2half_rn(__fadd_rn(lo[i], __fmul_rn(8.0f, s)));
+        off = __half2float(offset_h);
+        any = s > 0.0f;
+        inv = any ? __fdiv_rn(1.0f, s) : 0.0f;
+        if (t == 0 && to.tile)
+          reinterpret_cast<uint32_t *>(to.tile + 16 * D + (is_v ? 64 * ng : 0))[to.tok * ng + i / step_words] =
+              (uint32_t)__half_as_ushort(scale_h) | (uint32_t)__half_as_ushort(offset_h) << 16;
+      }
+      uint32_t w = 0;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float y = any ? rintf(__fmul_rn(__fsub_rn(x[i][e], off), inv)) : 0.0f;
+        const uint32_t code = (uint32_t)((int)fminf(fmaxf(y, -8.0f), 7.0f) + 8);
+        w |= code << (4 * (is_v ? e : (e & 1) * 4 + e / 2));
+      }
+      words[i] = w;
+    }
+    if (!is_v && to.tile) {
+#pragma unroll
+      for (int sl = 0; sl < kSlabs; ++sl)
+        store_words4<kWpr>(to.tile + ((sl * 16 + to.tok) * 4 + t) * kWpr * 4, words + sl * kWpr);
+    }
+  }
+  if (!is_v) return;
+  // V. Lane (e, p) is to have dims e + 8 {0, 1, 2, 3} of tokens 2 p and 2 p + 1.
+  uint32_t out[kWords];
+#pragma unroll
+  for (int i = 0; i < kWords; ++i) {
+    uint32_t w = 0;  // nibbles 2 t (low half) and 2 t + 1 of the four lanes' words
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const uint32_t b = __shfl_sync(0xffffffffu, words[i], (lane & 28) + q) >> (8 * t);
+      w |= (b & 15u) << (4 * q) | (b >> 4 & 15u) << (16 + 4 * q);
+    }
+    const uint32_t a = __shfl_sync(0xffffffffu, w, (2 * t) * 4 + g / 2);
+    const uint32_t b = __shfl_sync(0xffffffffu, w, (2 * t + 1) * 4 + g / 2);
+    out[i] = __byte_perm(a, b, g & 1 ? 0x7632 : 0x5410);
+  }
+  const Spot s0 = spot_of(mine, 2 * t), s1 = spot_of(mine, 2 * t + 1);
+  if (s0.tile && s0.tile == s1.tile && s1.tok == s0.tok + 1 && !(s0.tok & 1)) {  // a pair of the page
+#pragma unroll
+    for (int sl = 0; sl < kSlabs; ++sl)
+      store_words4<kWpr>(s0.tile + 8 * D + (((sl * 2 + s0.tok / 8) * 8 + g) * 4 + s0.tok % 8 / 2) * kWpr * 4,
+                         out + sl * kWpr);
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) word |= code[e] << (4 * e);
-  }
-  // V: nibbles g = 2t and 2t + 1 of the four lanes (dims 8 k + g)
-  uint32_t p0 = 0, p1 = 0;
+    for (int b = 0; b < 2; ++b) {
+      const Spot &s = b ? s1 : s0;
+      if (!s.tile) continue;
 #pragma unroll
-  for (int kk = 0; kk < 4; ++kk) {
-    const uint32_t w = __shfl_sync(0xffffffffu, word, (threadIdx.x & 28) + kk) >> (8 * t);
-    p0 |= (w & 15u) << (4 * kk);
-    p1 |= (w >> 4 & 15u) << (4 * kk);
+      for (int i = 0; i < kWords; ++i)
+        reinterpret_cast<uint16_t *>(s.tile + 8 * D)[((((i / kWpr * 2 + s.tok / 8) * 8 + g) * 4 + s.tok % 8 / 2) * kWpr +
+                                                      i % kWpr) * 2 + s.tok % 2] = (uint16_t)(out[i] >> (16 * b));
+    }
   }
-  if (!ok) return;
-  if (!is_v) {
-    *reinterpret_cast<uint32_t *>(tile + 4 * (((slab * 16 + tok) * 4 + t) * kWords + i)) = word;
-  } else {
-    const int p = tok / 8, vt = tok % 8 / 2, b = tok % 2;
-    uint16_t *at = reinterpret_cast<uint16_t *>(tile + 8 * D) + (((slab * 2 + p) * 8 * 4 + vt) * kWords + i) * 2 + b;
-    at[(2 * t) * 4 * kWords * 2] = (uint16_t)p0;
-    at[(2 * t + 1) * 4 * kWords * 2] = (uint16_t)p1;
-  }
-  if (lane % (group / 8) == 0)
-    reinterpret_cast<uint32_t *>(tile + 16 * D + (is_v ? 64 * ng : 0))[tok * ng + lane / (group / 8)] =
-        (uint32_t)__half_as_ushort(scale_h) | (uint32_t)__half_as_ushort(offset_h) << 16;
 }
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kTokenThreads)
     kv4_read_kernel(const Kv4View c, const int group, T *__restrict__ k, T *__restrict__ v, const bool vec,
                     const int64_t *__restrict__ slots, const int n) {
-  constexpr int kLanes = D / 8, kWords = (D < 128 ? D : 128) / 32;
-  const int64_t rows = (int64_t)n * 2 * c.kv_heads;
-  const int64_t id = (int64_t)blockIdx.x * kTokenThreads + threadIdx.x;
-  int64_t row = id / kLanes;
-  const int lane = (int)(id % kLanes);
-  const bool there = row < rows;
-  if (!there) row = rows - 1;
-  const int head = (int)(row % c.kv_heads);
-  const int64_t tk = row / c.kv_heads;
-  const bool is_v = tk & 1;
-  const int64_t token = tk >> 1;
-  const int64_t slot = __ldg(slots + token);
-  const int64_t page = slot >> c.page_log2;
-  const bool ok = slot >= 0 && page < c.num_pages;
-  if (there && slot >= 0 && !ok) kv4_error(c.errors, kErrBounds);
-  const int in_page = (int)(slot & (c.page_size - 1)), tok = in_page % kKv4Tile;
-  const int ng = D / group;
-  const uint8_t *tile = c.base + (ok ? page : 0) * c.page_stride + head * c.head_bytes +
-                        (uint64_t)(ok ? in_page / kKv4Tile : 0) * kv4_tile_bytes(D, group);
-  const int slab = lane / (kWords * 4), i = lane % (kWords * 4) / 4, t = lane % 4;
-  uint32_t word = 0, p0 = 0, p1 = 0;
-  if (!is_v) {
-    word = *reinterpret_cast<const uint32_t *>(tile + 4 * (((slab * 16 + tok) * 4 + t) * kWords + i));
-  } else {
-    const int p = tok / 8, vt = tok % 8 / 2, b = tok % 2;
-    const uint16_t *at =
-        reinterpret_cast<const uint16_t *>(tile + 8 * D) + (((slab * 2 + p) * 8 * 4 + vt) * kWords + i) * 2 + b;
-    p0 = at[(2 * t) * 4 * kWords * 2];
-    p1 = at[(2 * t + 1) * 4 * kWords * 2];
-  }
-  const uint32_t par = reinterpret_cast<const uint32_t *>(tile + 16 * D + (is_v ? 64 * ng : 0))[tok * ng + lane / (group / 8)];
-  const float s = kv4_scale(par), o = kv4_offset(par);
-  // V: lane t of the four holds nibbles of g = 2t, 2t + 1; it wants nibble t of every g
+  constexpr int kSlabs = D > 128 ? 2 : 1, kWpr = D / kSlabs / 32, kWords = D / 32;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, ng = D / group;
+  const int64_t id = (int64_t)blockIdx.x * (kTokenThreads / 32) + (threadIdx.x >> 5);
+  const int head = (int)(id % c.kv_heads);
+  const bool is_v = id / c.kv_heads & 1;
+  const int64_t first = id / c.kv_heads / 2 * kTokensWarp;
+  if (first >= n) return;
+  const Spot mine = load_spot(c, slots, n, first, head, kv4_tile_bytes(D, group));
+  const int step_words = group / 32;
+  {
+    const Spot at = spot_of(mine, g);
+    uint32_t w[kWords], par[kWords];
 #pragma unroll
-  for (int g2 = 0; g2 < 4; ++g2) {
-    const uint32_t a = __shfl_sync(0xffffffffu, p0, (threadIdx.x & 28) + g2);
-    const uint32_t b = __shfl_sync(0xffffffffu, p1, (threadIdx.x & 28) + g2);
-    if (is_v) word |= (a >> (4 * t) & 15u) << (8 * g2) | (b >> (4 * t) & 15u) << (8 * g2 + 4);
-  }
-  if (!there) return;
-  T y[8];
+    for (int i = 0; i < kWords; ++i) w[i] = par[i] = 0;
+    if (at.tile) {
+      const uint32_t *params = reinterpret_cast<const uint32_t *>(at.tile + 16 * D + (is_v ? 64 * ng : 0)) + at.tok * ng;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const int nib = is_v ? e : (e & 1) * 4 + e / 2;
-    y[e] = ok ? kv4_round<T>(kv4_value(word >> (4 * nib) & 15u, s, o)) : kv4_round<T>(0.0f);
-  }
-  T *dst = (is_v ? v : k) + (token * c.kv_heads + head) * D + lane * 8;
-  if (vec) {
+      for (int i = 0; i < kWords; ++i) par[i] = params[i / step_words];
+    }
+    if (!is_v) {
+      if (at.tile) {
 #pragma unroll
-    for (int w = 0; w < (int)sizeof(T) / 2; ++w)
-      reinterpret_cast<uint4 *>(dst)[w] = *reinterpret_cast<const uint4 *>(y + w * (16 / sizeof(T)));
-  } else {
+        for (int sl = 0; sl < kSlabs; ++sl)
+          load_words4<kWpr>(at.tile + ((sl * 16 + at.tok) * 4 + t) * kWpr * 4, w + sl * kWpr);
+      }
+    } else {
+      // a lane fetches words of tokens 2 t and 2 t + 1 (dims g + 8 {0 .. 3}), as they lie
+      const Spot s0 = spot_of(mine, 2 * t), s1 = spot_of(mine, 2 * t + 1);
+      uint32_t a[kWords], b[kWords];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) dst[e] = y[e];
+      for (int i = 0; i < kWords; ++i) a[i] = b[i] = 0;
+#pragma unroll
+      for (int sl = 0; sl < kSlabs; ++sl) {
+        if (s0.tile)
+          load_words4<kWpr>(s0.tile + 8 * D + (((sl * 2 + s0.tok / 8) * 8 + g) * 4 + s0.tok % 8 / 2) * kWpr * 4, a + sl * kWpr);
+        if (s1.tile)
+          load_words4<kWpr>(s1.tile + 8 * D + (((sl * 2 + s1.tok / 8) * 8 + g) * 4 + s1.tok % 8 / 2) * kWpr * 4, b + sl * kWpr);
+      }
+      const uint32_t pick = (s0.tok & 1 ? 0x32u : 0x10u) | (s1.tok & 1 ? 0x7600u : 0x5400u);
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) {
+        const uint32_t both = __byte_perm(a[i], b[i], pick);  // 4 nibbles (dims 8 apart) of each token
+        // lane (row, t) wants, of its row, nibble t of dims 0 .. 7: they are with the lanes
+        // (dim, row / 2), in the half row % 2
+        uint32_t y = 0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const uint32_t x = __shfl_sync(0xffffffffu, both, e * 4 + g / 2);
+          y |= (x >> (16 * (g & 1) + 4 * t) & 15u) << (4 * e);
+        }
+        w[i] = y;
+      }
+    }
+    if (first + g < n) {
+      T *dst = (is_v ? v : k) + ((first + g) * c.kv_heads + head) * D + 8 * t;
+#pragma unroll
+      for (int i = 0; i < kWords; ++i) {
+        const float s = kv4_scale(par[i]), o = kv4_offset(par[i]);
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int nib = is_v ? e : (e & 1) * 4 + e / 2;
+          x[e] = kv4_value(w[i] >> (4 * nib) & 15u, s, o);
+        }
+        store8(dst + 32 * i, vec, x);
+      }
+    }
   }
+}
+
+// A warp for 8 tokens, K or V, and head.
+inline uint64_t token_blocks(const Kv4View &c, int n) {
+  const uint64_t warps = ((uint64_t)n + kTokensWarp - 1) / kTokensWarp * 2 * c.kv_heads;
+  return (warps + kTokenThreads / 32 - 1) / (kTokenThreads / 32);
 }
 
 template <typename T, int D>
 cudaError_t launch_append(const Kv4View &c, int group, const void *k, const void *v, const TokenStrides &st,
                           const int64_t *slots, int n, cudaStream_t stream) {
-  const uint64_t threads = (uint64_t)n * 2 * c.kv_heads * (D / 8);
   const uint64_t unit = 16 / sizeof(T);
   const bool vec = ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) == 0 &&
                    ((st.k_token | st.k_head | st.v_token | st.v_head) & (int64_t)(unit - 1)) == 0;
-  kv4_append_kernel<T, D><<<(unsigned)((threads + kTokenThreads - 1) / kTokenThreads), kTokenThreads, 0, stream>>>(
+  kv4_append_kernel<T, D><<<(unsigned)token_blocks(c, n), kTokenThreads, 0, stream>>>(
       c, group, static_cast<const T *>(k), static_cast<const T *>(v), st, vec, slots, n);
   return cudaGetLastError();
 }
@@ -424,9 +566,8 @@ cudaError_t launch_append(const Kv4View &c, int group, const void *k, const void
 template <typename T, int D>
 cudaError_t launch_read(const Kv4View &c, int group, void *k, void *v, const int64_t *slots, int n,
                         cudaStream_t stream) {
-  const uint64_t threads = (uint64_t)n * 2 * c.kv_heads * (D / 8);
   const bool vec = ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) == 0;
-  kv4_read_kernel<T, D><<<(unsigned)((threads + kTokenThreads - 1) / kTokenThreads), kTokenThreads, 0, stream>>>(
+  kv4_read_kernel<T, D><<<(unsigned)token_blocks(c, n), kTokenThreads, 0, stream>>>(
       c, group, static_cast<T *>(k), static_cast<T *>(v), vec, slots, n);
   return cudaGetLastError();
 }
@@ -445,9 +586,7 @@ cudaError_t by_form(int dtype, int d, F f) {
 }
 
 // The last grid index of a launch over n tokens has to stay inside 31 bits.
-bool tokens_fit(const cb_kv4_cache *c, int32_t n) {
-  return (uint64_t)n * 2 * c->kv_heads * (c->head_dim / 8) / kTokenThreads < 0x7fffffffull;
-}
+bool tokens_fit(const Kv4View &c, int32_t n) { return token_blocks(c, n) < 0x7fffffffull; }
 
 }  // namespace
 
@@ -473,7 +612,14 @@ extern "C" int cb_kv4_plan(const cb_kv4_plan_args *a, void *stream) {
   Kv4Device dev(a->device);
   if (dev.err != cudaSuccess) return kv4_fail(CB_ERR_CUDA, "cb_kv4_plan: device", dev.err);
   int ctas = 1;
+  // 16,384 tokens: one run of 32 for every warp of the largest cluster
+  const bool many = a->tokens > 2 * kPlanCtas * kPlanThreads;
   while (ctas < kPlanCtas && a->tokens > ctas * 2 * kPlanThreads) ctas *= 2;
+  const auto kernel = many ? kv4_plan_kernel<kPlanRun> : kv4_plan_kernel<1>;
+  if (ctas > 8) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (e != cudaSuccess) return kv4_fail(CB_ERR_CUDA, "cb_kv4_plan: cluster size", e);
+  }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(ctas);
   cfg.blockDim = dim3(kPlanThreads);
@@ -483,8 +629,8 @@ extern "C" int cb_kv4_plan(const cb_kv4_plan_args *a, void *stream) {
   at[0].val.clusterDim.x = ctas;
   at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, kv4_plan_kernel, *a, ctas);
+  cfg.numAttrs = ctas > 1 ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, *a, ctas);
   return e == cudaSuccess ? CB_OK : kv4_fail(CB_ERR_CUDA, "cb_kv4_plan: launch", e);
 }
 
@@ -496,7 +642,7 @@ extern "C" int cb_kv4_append(const cb_kv4_cache *cache, int32_t layer, int32_t d
   if (int rc = kv4_check_cache(cache, layer, "cb_kv4_append: no cache", &c)) return rc;
   if (dtype < CB_KV4_F16 || dtype > CB_KV4_F32) return kv4_fail(CB_ERR_ARG, "cb_kv4_append: unknown dtype");
   if (n < 0 || (n > 0 && (!k || !v || !slots))) return kv4_fail(CB_ERR_ARG, "cb_kv4_append: bad arguments");
-  if (!tokens_fit(cache, n)) return kv4_fail(CB_ERR_ARG, "cb_kv4_append: too many tokens in one call");
+  if (!tokens_fit(c, n)) return kv4_fail(CB_ERR_ARG, "cb_kv4_append: too many tokens in one call");
   if (n == 0) return CB_OK;
   Kv4Device dev(cache->device);
   if (dev.err != cudaSuccess) return kv4_fail(CB_ERR_CUDA, "cb_kv4_append: device", dev.err);
@@ -515,7 +661,7 @@ extern "C" int cb_kv4_read(const cb_kv4_cache *cache, int32_t layer, int32_t dty
   if (int rc = kv4_check_cache(cache, layer, "cb_kv4_read: no cache", &c)) return rc;
   if (dtype < CB_KV4_F16 || dtype > CB_KV4_F32) return kv4_fail(CB_ERR_ARG, "cb_kv4_read: unknown dtype");
   if (n < 0 || (n > 0 && (!k_out || !v_out || !slots))) return kv4_fail(CB_ERR_ARG, "cb_kv4_read: bad arguments");
-  if (!tokens_fit(cache, n)) return kv4_fail(CB_ERR_ARG, "cb_kv4_read: too many tokens in one call");
+  if (!tokens_fit(c, n)) return kv4_fail(CB_ERR_ARG, "cb_kv4_read: too many tokens in one call");
   if (n == 0) return CB_OK;
   Kv4Device dev(cache->device);
   if (dev.err != cudaSuccess) return kv4_fail(CB_ERR_CUDA, "cb_kv4_read: device", dev.err);

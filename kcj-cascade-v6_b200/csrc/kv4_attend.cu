@@ -739,8 +739,8 @@ int sm_count(int device) {
 template <int D, int NG, int NT>
 cudaError_t run_few(const Kv4View &c, const AttendArgs &a, const Launch &l, cudaStream_t stream) {
   using F = Form<D, NG, NT>;
-  cudaError_t e =
-      cudaFuncSetAttribute(attend_few_kernel<D, NG, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem);
+  static std::atomic<uint64_t> ready{0};  // a bit for each device
+  cudaError_t e = allow_shared(attend_few_kernel<D, NG, NT>, F::kSmem, ready);
   if (e != cudaSuccess) return e;
   attend_few_kernel<D, NG, NT><<<l.pieces / kWarps, kThreads, F::kSmem, stream>>>(c, a);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
@@ -786,9 +786,11 @@ int few_tiles(int head_dim, int64_t rows) {
 }
 
 // Above this many rows of a request the prompt kernel takes it (where it is
-// offered: head_dim 64 and 128); the few-row kernel would read the cache once for
-// every 32 rows.
-constexpr int kFewRows = 32;
+// offered: head_dim 64 and 128). It works on 128 rows whether there are or not, the
+// few-row kernel reads the cache once for every 32. 24 requests of up to 7,000
+// tokens, 8 KV heads of 128, few-row against prompt kernel: 64 rows 139 against 180
+// us, 96 rows 197 against 186, 128 rows 252 against 186.
+constexpr int kFewRows = 64;
 
 struct Launches {
   Launch few, prompt;

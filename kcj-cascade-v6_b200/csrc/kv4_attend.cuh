@@ -9,6 +9,7 @@
 // which only the device knows.
 #pragma once
 
+#include <atomic>
 #include <type_traits>
 
 #include "kv4.cuh"
@@ -52,6 +53,19 @@ struct Launch {
   int sms, pieces;
   int part;  // floats of a partial result
 };
+
+// Lets a kernel use `bytes` of shared memory on the current device, once for each.
+template <typename K>
+cudaError_t allow_shared(K kernel, int bytes, std::atomic<uint64_t> &ready) {
+  int device = 0;
+  cudaError_t e = cudaGetDevice(&device);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = device < 64 ? 1ull << device : 0;
+  if (ready.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) ready.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
 
 inline uint64_t launch_bytes(const Launch &l) {
   return ((uint64_t)l.pieces * (sizeof(int4) + 2ull * sizeof(float) * l.part + sizeof(int) + 1) + 16 + 15) / 16 * 16;

@@ -735,8 +735,8 @@ template <int D, int NG>
 cudaError_t launch(const Kv4View &c, const AttendArgs &a, const Launch &l, cudaStream_t stream) {
   using F = PromptForm<D, NG>;
   static_assert(F::kSmem <= 227 * 1024 && kBarCount * 8 <= 256, "shared memory");
-  cudaError_t e =
-      cudaFuncSetAttribute(attend_prompt_kernel<D, NG>, cudaFuncAttributeMaxDynamicSharedMemorySize, F::kSmem);
+  static std::atomic<uint64_t> ready{0};  // a bit for each device
+  cudaError_t e = allow_shared(attend_prompt_kernel<D, NG>, F::kSmem, ready);
   if (e != cudaSuccess) return e;
   attend_prompt_kernel<D, NG><<<l.pieces, kPromptThreads, F::kSmem, stream>>>(c, a);
   if ((e = cudaGetLastError()) != cudaSuccess) return e;
