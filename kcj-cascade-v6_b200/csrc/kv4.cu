@@ -98,7 +98,8 @@ CB_D long long block_scan(long long x, long long *warp_sums, long long &total) {
 }
 
 // Last index i in [0, n) with start[i] <= e (start ascending, start[0] <= e).
-CB_D int find_row(const long long *start, int n, long long e) {
+template <typename I>
+CB_D int find_row(const I *start, int n, I e) {
   int lo = 0, hi = n;
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
@@ -115,13 +116,14 @@ CB_D void plan_barrier(int ctas) {
 
 template <int RUN>
 __global__ void __launch_bounds__(kPlanThreads) kv4_plan_kernel(const cb_kv4_plan_args a, const int ctas) {
-  __shared__ long long start[kPlanThreads + 1], base[kPlanThreads], warp_sums[kPlanThreads / 32];
+  __shared__ long long start[kPlanThreads], warp_sums[kPlanThreads / 32];
+  __shared__ int begin_s[kPlanThreads], base_s[kPlanThreads];
   __shared__ int len_s[kPlanThreads], held_s[kPlanThreads];  // held_s: -1 for a refused row
   const int tid = threadIdx.x, lane = tid & 31;
   const long long stride = (long long)ctas * kPlanThreads * RUN;  // of the cluster
   const int rank = ctas > 1 ? (int)cg::this_cluster().block_rank() : 0;
   const long long mine = ((long long)rank * kPlanThreads + (tid & ~31)) * RUN + lane;
-  const int ps = a.page_size;
+  const int ps = a.page_size, log2 = (ps & (ps - 1)) == 0 ? 31 - __clz(ps) : -1;
   const long long most = (long long)a.columns * ps;
   long long count = min(max(*a.free_count, 0), a.num_pages);
 
@@ -193,8 +195,8 @@ __global__ void __launch_bounds__(kPlanThreads) kv4_plan_kernel(const cb_kv4_pla
     const bool ok = fits && (need == 0 || first + need <= count);
     long long used_total;
     block_scan(ok ? need : 0, warp_sums, used_total);
-    start[tid] = at;
-    base[tid] = first;
+    begin_s[tid] = (int)min(at, 0x7fffffffll);
+    base_s[tid] = (int)min(first, 0x7fffffffll);
     len_s[tid] = (int)len;
     held_s[tid] = ok ? held : -1;
     if (rank == 0 && r < a.requests) {
@@ -202,40 +204,44 @@ __global__ void __launch_bounds__(kPlanThreads) kv4_plan_kernel(const cb_kv4_pla
       a.status[r] = ok ? CB_PUT_STORED : CB_PUT_FAILED;
     }
     __syncthreads();
-    const long long end = min(tokens + total, (long long)a.tokens);
-    for (long long n0 = tokens + mine; n0 - lane < end; n0 += stride) {
+    const int end = (int)min(tokens + total, (long long)a.tokens);
+    for (long long n0_ = tokens + mine; n0_ - lane < end; n0_ += stride) {
+      const int n0 = (int)min(n0_, 0x7fffffffll);
       int page[RUN], pos[RUN], row[RUN];
-      int i = n0 < end ? find_row(start, kPlanThreads, n0) : 0;
+      int i = n0 < end ? find_row(begin_s, kPlanThreads, n0) : 0;
+      int next = i + 1 < kPlanThreads ? begin_s[i + 1] : 0x7fffffff;
 #pragma unroll
       for (int u = 0; u < RUN; ++u) {
-        const long long n = n0 + 32 * u;
-        while (n < end && i + 1 < kPlanThreads && start[i + 1] <= n) ++i;
+        const int n = n0 + 32 * u;
         page[u] = -1, pos[u] = 0, row[u] = -1;
-        if (n < end) {
-          const long long p = len_s[i] + (n - start[i]);
-          pos[u] = (int)min(p, 0x7fffffffll);
-          if (held_s[i] >= 0) {
-            const int col = pos[u] / ps;
+        if (n0 < end && 32 * u < end - n0) {
+          while (next <= n) {
+            ++i;
+            next = i + 1 < kPlanThreads ? begin_s[i + 1] : 0x7fffffff;
+          }
+          pos[u] = (int)min((uint32_t)len_s[i] + (uint32_t)(n - begin_s[i]), 0x7fffffffu);
+          const int held = held_s[i];
+          if (held >= 0) {
+            const int col = log2 >= 0 ? pos[u] >> log2 : pos[u] / ps;
             row[u] = i;
-            page[u] = col < held_s[i] ? a.block_table[(r0 + i) * a.table_stride + col]
-                                      : a.free[count - 1 - (base[i] + col - held_s[i])];
+            page[u] = col < held ? a.block_table[(r0 + i) * a.table_stride + col]
+                                 : a.free[(int)count - 1 - (base_s[i] + col - held)];
           }
         }
       }
 #pragma unroll
       for (int u = 0; u < RUN; ++u) {
-        const long long n = n0 + 32 * u;
-        if (n >= end) break;
+        if (n0 >= end || 32 * u >= end - n0) break;
         long long slot = -1;
         if (row[u] >= 0) {
-          const int col = pos[u] / ps, in_page = pos[u] - col * ps;
+          const int col = log2 >= 0 ? pos[u] >> log2 : pos[u] / ps, in_page = pos[u] - col * ps;
           if (in_page == 0 && col >= held_s[row[u]])  // the first token of a new page
             a.block_table[(r0 + row[u]) * a.table_stride + col] = page[u];
           if (page[u] >= 0 && page[u] < a.num_pages) slot = (long long)page[u] * ps + in_page;
           else kv4_error(a.errors, kErrBounds);
         }
-        a.slots[n] = slot;
-        a.positions[n] = pos[u];
+        a.slots[n0 + 32 * u] = slot;
+        a.positions[n0 + 32 * u] = pos[u];
       }
     }
     tokens += total;
