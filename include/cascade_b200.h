@@ -419,7 +419,8 @@ int cb_hash_batch_noalloc(int32_t device, const void *const *ptrs, const uint64_
 #define CB_KV4_F16 0
 #define CB_KV4_BF16 1
 #define CB_KV4_F32 2
-#define CB_KV4_ERROR_RANGE 1 /* bit of *errors: slot, page or length out of range */
+#define CB_KV4_ERROR_RANGE 1   /* bits of *errors: slot, page or length out of range */
+#define CB_KV4_ERROR_TIMEOUT 2 /* a wait inside a kernel ran out (results are void)  */
 
 typedef struct cb_kv4_cache {
   void *pages;          /* 16-byte aligned                                   */
@@ -487,10 +488,10 @@ int cb_kv4_read(const cb_kv4_cache *cache, int32_t layer, int32_t dtype, void *k
  * [total_q][q_heads][head_dim] and the tokens 0 .. kv_lens[i] of its pages
  * block_table[i][..]; row r of its n rows sees the tokens below kv_len - (n -
  * 1 - r) when causal, else all of them. q_heads is a multiple of kv_heads. A
- * row that sees nothing gets zeros and lse -inf; columns * page_size is at most
- * 2^30. out: [total_q][q_heads]
- * [head_dim] dense, 16-byte aligned, of q's type; lse (natural log, [total_q][q_heads] fp32) or
- * NULL. Rows behind q_start[requests] are left as they were. max_q is a hint
+ * row that sees nothing gets zeros and lse -inf; one that sees a NaN gets NaN.
+ * columns * page_size is at most 2^30. out: [total_q][q_heads][head_dim] dense,
+ * 16-byte aligned, of q's type, not overlapping q; lse (natural log,
+ * [total_q][q_heads] fp32) or NULL. Rows behind q_start[requests] are left as they were. max_q is a hint
  * (rows of a request at most); results do not depend on it being right.
  * workspace: cb_kv4_attend_workspace bytes, 16-byte aligned, used until the
  * call's work is done. */

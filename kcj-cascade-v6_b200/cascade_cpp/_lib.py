@@ -47,6 +47,7 @@ CB_KV4_F16 = 0
 CB_KV4_BF16 = 1
 CB_KV4_F32 = 2
 CB_KV4_ERROR_RANGE = 1
+CB_KV4_ERROR_TIMEOUT = 2
 
 
 class cb_config(C.Structure):

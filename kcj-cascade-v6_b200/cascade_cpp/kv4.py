@@ -202,7 +202,8 @@ class KV4Cache(KVPageConnector):
         ``[requests + 1]``; without it, one row each) and the first
         ``kv_lens[i]`` tokens of its pages ``block_table[i]``. When ``causal``,
         its last row sees every token and each row before it one fewer; a row
-        that sees nothing gets zeros (log-sum-exp -inf). Query heads are in
+        that sees nothing gets zeros (log-sum-exp -inf), one that sees a NaN
+        NaN. Query heads are in
         groups of q_heads / kv_heads that share a KV head. ``scale`` defaults
         to 1 / sqrt(head_dim). ``max_q`` (rows of a request at most) only helps
         the choice of kernel. Rows behind the last request are left as they
@@ -239,12 +240,14 @@ class KV4Cache(KVPageConnector):
         lse = torch.empty((rows, heads), dtype=torch.float32, device=dev) if return_lse else None
         a = L.cb_kv4_attend_args(
             q.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(), block_table.data_ptr(), lens,
-            start, None, 0, max(block_table.stride(0), columns), q.stride(0), q.stride(1),
+            start, None, 0, block_table.stride(0), q.stride(0), q.stride(1),
             d ** -0.5 if scale is None else scale, layer, code, n, columns, rows, heads,
             (1 if start is None else rows) if max_q is None else max_q, causal, 0)
         lib = _native_lib()
         need = self._work.get((heads, a.max_q))  # the sizes that decide it
         if need is None:
+            if len(self._work) > 255:
+                self._work.clear()
             need = self._work[heads, a.max_q] = lib.cb_kv4_attend_workspace(self._form, a)
         work = torch.empty(need, dtype=torch.uint8, device=dev)
         a.workspace, a.workspace_bytes = work.data_ptr(), need
@@ -257,6 +260,8 @@ class KV4Cache(KVPageConnector):
         bits = int(self.errors.item())
         if bits:
             self.errors.zero_()
+            if bits & L.CB_KV4_ERROR_TIMEOUT:
+                raise CascadeError(L.CB_ERR_TIMEOUT, "a wait inside a kernel ran out")
             raise CascadeError(L.CB_ERR_DEVICE, "a slot, page or length was outside the cache")
 
 
@@ -366,7 +371,7 @@ class PageTable:
         ``borrowed`` the pages stay someone else's (a prefix that several rows
         share): they do not go to the free stack when the row is done. Further
         tokens go to pages of the row's own, so ``tokens`` must then fill the
-        pages."""
+        pages. Waits for the GPU."""
         if not 0 <= row < self.requests:
             raise IndexError("row out of range")
         n, tokens = len(pages), int(tokens)
@@ -376,6 +381,8 @@ class PageTable:
             raise ValueError("a borrowed page must be full")
         if n and (min(pages) < 0 or max(pages) >= self.num_pages):
             raise IndexError("page index out of range")
+        if int(self.kv_lens[row]):
+            raise ValueError("the row is not empty")
         if n:
             self.block_table[row, :n] = torch.tensor(list(pages), dtype=torch.int32, device=self.device)
         self.kv_lens[row] = tokens

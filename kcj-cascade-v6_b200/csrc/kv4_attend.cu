@@ -12,8 +12,10 @@ namespace {
 
 // Row tiles of 8*NT rows (query row x query head of one KV head), tokens in
 // tiles of 16, a piece of the line (kv4_attend.cuh) for every WARP: warps share
-// nothing and never wait for one another. An item that ends up in several warps leaves partial sums in the
-// workspace, joined by a second kernel in a fixed order.
+// nothing and never wait for one another. (With a piece for every block, whose
+// warps met at each item's end, 61 ragged requests took 53 us instead of 49.) An
+// item that ends up in several warps leaves partial sums in the workspace, joined
+// by a second kernel in a fixed order.
 //
 // Tensor-core form (16x8x16, fp16 in, fp32 sums): the cache is the 16-row
 // operand of both products and the 8*NT query rows the 8-wide one, so that the
@@ -30,13 +32,23 @@ namespace {
 // is the one that the centring by 8 uses) and the output. q is brought to fp16
 // by a power of two per row: exact for fp16 and, above 2^-28 of the row's
 // largest, for bf16.
+//
+// Bound by HBM where the tokens are many: 1 + 8/group bytes for a cached value pair
+// of K and V. Measured: 48 requests of 9,000 to 32,000 tokens, 64 / 8 heads of 128,
+// group 128: 214 us, 5.0 TB/s; the rest of the way is instructions (266 for a tile
+// of 16 tokens, 16 of them products and 80 the unpacking, at 0.6 an SM quarter and
+// cycle). A single short request is bound by latency: 11.4 us for 1,100 tokens.
+// mma.sync and not tcgen05: its operands come from registers, where the codes become
+// them with one instruction for two values, and 8 rows leave 15/16 of a 128-row
+// product empty; kv4_prompt.cu has the rows for that.
 constexpr int kWarps = 8, kThreads = kWarps * 32;
 constexpr int kRecentre = 4;      // pairs of tiles between centrings of the sums
+constexpr int kManyParts = 24;    // parts of an item that a warp joins alone
 // What an item costs a warp beside its tiles (query rows in, results out), in
 // tiles: it takes this much of the line too.
+// (130 requests of up to 3,000 tokens, 64 dims: 66 us with 3, 59 with 5 or 8.)
 constexpr int kItemCost = 8;
 constexpr int kJoinWarps = 8, kJoinThreads = kJoinWarps * 32;
-constexpr int kManyParts = 24;
 
 template <int D, int NG, int NT>
 struct Form {
@@ -48,7 +60,9 @@ struct Form {
   static constexpr int kGroupWords = kWords / NG;
   // A warp's ring is two pairs of tiles. Bytes in flight: 8 or 16 warps with 2 to 4
   // tiles of 1.2 - 5.1 KB are 35 KB and more on an SM; HBM needs about
-  // 6.5 TB/s * 0.8 us / 148 = 35 KB.
+  // 6.5 TB/s * 0.8 us / 148 = 35 KB. Products of two tiles side by side (kJoint)
+  // hide each other's latency where registers allow: 275 us without, 220 with, on
+  // the 48 long requests.
   static constexpr int kJoint = NT == 1 ? 2 : 1;  // tiles whose products run side by side
   static constexpr int kCtasPerSm = NT == 1 && D <= 128 ? 2 : 1;
   static constexpr int kRing = 4 * kTile;           // of a warp, as are the next two
@@ -817,7 +831,7 @@ int check(const cb_kv4_cache *cache, const cb_kv4_attend_args *a, Kv4View *c) {
   if (int rc = kv4_check_cache(cache, a->layer, "cb_kv4_attend: no cache", c)) return rc;
   if (a->dtype != CB_KV4_F16 && a->dtype != CB_KV4_BF16)
     return kv4_fail(CB_ERR_ARG, "cb_kv4_attend: q must be fp16 or bf16");
-  if (a->requests < 0 || a->columns <= 0 || a->total_q < 0 || a->q_heads <= 0 || a->table_stride < a->columns)
+  if (a->requests < 0 || a->columns <= 0 || a->total_q < 0 || a->q_heads <= 0 || a->table_stride < 0)
     return kv4_fail(CB_ERR_ARG, "cb_kv4_attend: bad sizes");
   if (a->q_heads % cache->kv_heads) return kv4_fail(CB_ERR_ARG, "cb_kv4_attend: q_heads is not a multiple of kv_heads");
   if ((long long)a->total_q * a->q_heads > 0x3fffffffll) return kv4_fail(CB_ERR_ARG, "cb_kv4_attend: too many rows");

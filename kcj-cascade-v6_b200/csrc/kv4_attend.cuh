@@ -19,6 +19,7 @@ namespace cb {
 constexpr float kSlack = 8.0f;  // p may reach 2^8 before a running maximum is raised
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr uint64_t kWaitNs = 2000000000ull;  // the longest wait on a barrier
+// How an item's parts are joined: not at all, a warp for 16 dims, a block for them.
 constexpr int kJoinNone = 0, kJoinFew = 1, kJoinMany = 2;
 
 struct AttendArgs {

@@ -15,6 +15,14 @@
 // A running maximum is raised only when a score passes it by 2^8, which seldom
 // happens after a row's first tokens, so that O is seldom rescaled.
 //
+// Measured: chunks of 900 to 1,537 tokens behind 5,200 to 9,100 cached ones, 64 / 8
+// heads of 128, bf16: 652 us, 745 TFLOP/s. The tensor cores are busy a third of the
+// time: 128 x 128 products from shared memory take about 84 cycles for 16 steps
+// instead of 64, and between a tile's scores and its weights lie about 2,500
+// cycles of one warp's latencies, which the other row tile's products only half
+// cover. Tried without gain: 8 dequantising warps, half of the exponentials as
+// polynomials, the weights handed over in two halves.
+//
 // Roundings to 16 bits: K and V as dequantised (2^-11 of a value; the price of one
 // product for a score, where exact codes would need one for every group and two
 // multiplications for every score), P, and the output; q is exact, as in

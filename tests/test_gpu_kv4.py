@@ -210,6 +210,9 @@ def test_a_dry_plan_leaves_the_table_and_a_borrowed_prefix_its_owner():
         t.attach(0, [1], 12, borrowed=True)
     with pytest.raises(IndexError):
         t.attach(3, [], 0)
+    t.attach(1, [4], 9)
+    with pytest.raises(ValueError):
+        t.attach(1, [5], 3)  # not empty
 
 
 def test_a_table_set_wrongly_is_reported_and_harms_nothing():
@@ -409,6 +412,37 @@ def test_q_with_nan_or_infinity_keeps_to_its_rows():
         keep = torch.ones(n, 8, dtype=torch.bool, device=DEV)
         keep[1, 3] = keep[0, 6] = False
         assert torch.equal(got[keep], want[keep])
+
+
+@pytest.mark.parametrize("n,ratio", [(3, 2), (100, 4)])  # the kernels for few and for many rows
+@pytest.mark.parametrize("which", [0, 1])
+def test_a_token_that_is_nan_stays_hidden_from_the_rows_before_it(n, ratio, which):
+    cache, _ = make(16, 1, 1, 128, 16, 64, seed=6)
+    table = torch.randperm(16, device=DEV).to(torch.int32).view(1, 16)
+    lens = torch.tensor([250], dtype=torch.int32, device=DEV)
+    start = torch.tensor([0, n], dtype=torch.int32, device=DEV)
+    q = torch.randn(n, ratio, 128, device=DEV).bfloat16()
+    want = cache.attend(0, q, table, lens, q_start=start)
+    # the token that the last two rows see, behind what the others do
+    slot = torch.tensor([int(table[0, 248 // 16]) * 16 + 248 % 16], device=DEV)
+    kv = [torch.randn(1, 1, 128, device=DEV), torch.randn(1, 1, 128, device=DEV)]
+    kv[which][:] = float("nan")
+    cache.append(0, *kv, slot)
+    got, lse = cache.attend(0, q, table, lens, q_start=start, return_lse=True)
+    assert torch.equal(got[:-2], want[:-2]) and torch.isfinite(lse[:-2]).all()
+    assert torch.isnan(got[-2:]).all()
+
+
+def test_requests_may_share_one_row_of_a_table():
+    cache, _ = make(4, 1, 2, 64, 16, 32, seed=1)
+    table = torch.tensor([[2, 0, 3]], dtype=torch.int32, device=DEV)
+    lens = torch.tensor([5, 40, 48], dtype=torch.int32, device=DEV)
+    q = torch.randn(3, 4, 64, device=DEV).half()
+    want = cache.attend(0, q, table.repeat(3, 1), lens)
+    assert torch.equal(cache.attend(0, q, table.expand(3, 3), lens), want)
+    wide = torch.zeros(3, 50, dtype=torch.int32, device=DEV)
+    wide[:, 7:10] = table
+    assert torch.equal(cache.attend(0, q, wide[:, 7:10], lens), want)
 
 
 def test_a_cache_past_4_gib():

@@ -92,7 +92,7 @@ def test_c_entry_points_refuse_before_they_touch_a_gpu():
                  q_head_stride=128, scale=1.0, layer=0, dtype=0, requests=2, columns=3, total_q=2, q_heads=8, max_q=1)
         return lib.cb_kv4_attend(c, L.cb_kv4_attend_args(**{**a, **kw}), None)
 
-    for kw in (dict(dtype=2), dict(q_heads=6), dict(q_heads=0), dict(columns=0), dict(table_stride=2), dict(total_q=3),
+    for kw in (dict(dtype=2), dict(q_heads=6), dict(q_heads=0), dict(columns=0), dict(table_stride=-1), dict(total_q=3), dict(out=8200),
                dict(q=None), dict(out=None), dict(kv_lens=None), dict(layer=5), dict(requests=-1),
                dict(columns=1 << 28, table_stride=1 << 28)):
         assert attend(**kw) == L.CB_ERR_ARG, kw
