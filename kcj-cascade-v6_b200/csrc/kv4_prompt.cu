@@ -16,12 +16,15 @@
 // happens after a row's first tokens, so that O is seldom rescaled.
 //
 // Measured: chunks of 900 to 1,537 tokens behind 5,200 to 9,100 cached ones, 64 / 8
-// heads of 128, bf16: 652 us, 745 TFLOP/s. The tensor cores are busy a third of the
-// time: 128 x 128 products from shared memory take about 84 cycles for 16 steps
-// instead of 64, and between a tile's scores and its weights lie about 2,500
-// cycles of one warp's latencies, which the other row tile's products only half
-// cover. Tried without gain: 8 dequantising warps, half of the exponentials as
-// polynomials, the weights handed over in two halves.
+// heads of 128, bf16: 657 us, 740 TFLOP/s. The tensor cores are busy a third of the
+// time, and what stands in their way is shared memory: for two row tiles the products
+// read 192 KB of operands a tile of tokens and the dequantising warps store 64 KB, 2,000
+// cycles of its bandwidth at best; of the 5,000 that a tile takes, a dequantising
+// warp spends 4,000 in its stores' queue (with that work left out, a tile takes
+// 4,000, with the softmax left out too, 3,600). Pairs of SMs that share a product
+// would halve the reads of K and V and their stores. Tried without gain: 8
+// dequantising warps, half of the exponentials as polynomials, the weights handed
+// over in two halves, no pass for the maximum.
 //
 // Roundings to 16 bits: K and V as dequantised (2^-11 of a value; the price of one
 // product for a score, where exact codes would need one for every group and two
