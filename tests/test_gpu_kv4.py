@@ -352,6 +352,31 @@ def test_attend_many_rows():
     attend_case("bf16", 64, 64, 16, 1, 2, lens, [1] * 300, seed=2, one_row=True)
 
 
+def test_attend_a_prompt_behind_a_long_prefix():
+    attend_case("bf16", 128, 128, 64, 1, 1, [6100], [70], seed=3)
+
+
+def test_attend_many_requests_of_both_kinds():
+    # single tokens beside chunks (each kernel takes its own), more requests than a block has threads
+    rng = np.random.default_rng(4)
+    qs = rng.choice([0, 1, 2, 17], 540).tolist()
+    lens = [int(q + rng.integers(0, 25)) for q in qs]
+    attend_case("fp16", 64, 64, 16, 1, 4, lens, qs, seed=4, max_q=17)
+
+
+@pytest.mark.parametrize("rows", [2, 90])
+def test_q_may_lie_on_odd_addresses(rows):
+    cache, _ = make(8, 1, 2, 128, 16, 64, seed=3)
+    table = torch.arange(8, dtype=torch.int32, device=DEV).view(1, 8)
+    lens = torch.tensor([125], dtype=torch.int32, device=DEV)
+    start = torch.tensor([0, rows], dtype=torch.int32, device=DEV)
+    q = torch.randn(rows, 6, 128, device=DEV).bfloat16()
+    odd = torch.empty(rows * 6 * 131 + 1, dtype=q.dtype, device=DEV)[1:].view(rows, 6, 131)[:, :, :128]
+    odd.copy_(q)
+    want = cache.attend(0, q, table, lens, q_start=start)
+    assert torch.equal(cache.attend(0, odd, table, lens, q_start=start), want)
+
+
 @pytest.mark.parametrize("wide,scale", [(300.0, None), (1e-3, None), (1.0, 0.0), (1.0, -0.5), (2e-6, 3e4)])
 def test_attend_large_and_tiny_scores(wide, scale):
     attend_case("bf16", 128, 64, 16, 2, 4, [100, 65], [1, 40], seed=4, wide=wide, scale=scale)
