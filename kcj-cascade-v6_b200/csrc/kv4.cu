@@ -315,6 +315,20 @@ CB_D void store8(T *p, bool vec, const float *x) {
   }
 }
 
+CB_D float max_nan(float x, float y) {
+  float v;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(v) : "f"(x), "f"(y));
+  return v;
+}
+
+// x / 15, correctly rounded: a product with the rounded reciprocal, corrected once by
+// its exact remainder (Markstein). x is 0 or far above the smallest normal number.
+CB_D float fifteenth(float x) {
+  constexpr float r = 1.0f / 15.0f;
+  const float q = __fmul_rn(x, r);
+  return __fmaf_rn(__fmaf_rn(-15.0f, q, x), r, q);
+}
+
 struct TokenStrides {
   int64_t k_token, k_head, v_token, v_head;
 };
@@ -368,72 +382,72 @@ CB_D void store_words4(void *p, const uint32_t *w) {
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kTokenThreads)
-    kv4_append_kernel(const Kv4View c, const int group, const T *__restrict__ k, const T *__restrict__ v,
+    kv4_append_kernel(const Kv4View c, const int group_log2, const T *__restrict__ k, const T *__restrict__ v,
                       const TokenStrides st, const bool vec, const int64_t *__restrict__ slots, const int n) {
   constexpr int kSlabs = D > 128 ? 2 : 1, kWpr = D / kSlabs / 32, kWords = D / 32;
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, ng = D / group;
-  const int64_t id = (int64_t)blockIdx.x * (kTokenThreads / 32) + (threadIdx.x >> 5);
-  const int head = (int)(id % c.kv_heads);
-  const bool is_v = id / c.kv_heads & 1;
-  const int64_t first = id / c.kv_heads / 2 * kTokensWarp;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int group = 1 << group_log2, ng = D >> group_log2;
+  const uint32_t id = blockIdx.x * (kTokenThreads / 32) + (threadIdx.x >> 5), part = id / (uint32_t)c.kv_heads;
+  const int head = (int)(id - part * c.kv_heads);
+  const bool is_v = part & 1;
+  const int64_t first = (int64_t)(part >> 1) * kTokensWarp;
   if (first >= n) return;
-  const Spot mine = load_spot(c, slots, n, first, head, kv4_tile_bytes(D, group));
+  const Spot mine = load_spot(c, slots, n, first, head, 16 * D + 128 * ng);
   uint32_t words[kWords];  // codes of token g: dims 8 t + e of block i in nibble e
   {
     const Spot to = spot_of(mine, g);
     const int64_t row = first + (first + g < n ? g : 0);
     const T *src = (is_v ? v + row * st.v_token + head * st.v_head : k + row * st.k_token + head * st.k_head) + 8 * t;
-    float x[kWords][8], lo[kWords], hi[kWords], nan[kWords];
+    float x[kWords][8], lo[kWords], hi[kWords];
 #pragma unroll
     for (int i = 0; i < kWords; ++i) load8(src + 32 * i, vec, x[i]);
 #pragma unroll
     for (int i = 0; i < kWords; ++i) {
-      // fmin and fmax drop a NaN: it is carried beside them
-      lo[i] = INFINITY, hi[i] = -INFINITY, nan[i] = 0.0f;
+      lo[i] = INFINITY, hi[i] = -INFINITY;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        if (x[i][e] != x[i][e]) nan[i] = x[i][e];
-        x[i][e] = fminf(fmaxf(x[i][e], -kKv4Most), kKv4Most);
         lo[i] = fminf(lo[i], x[i][e]);
-        hi[i] = fmaxf(hi[i], x[i][e]);
+        hi[i] = max_nan(hi[i], x[i][e]);  // a NaN stays, and makes the scale NaN
+        x[i][e] = fminf(fmaxf(x[i][e], -kKv4Most), kKv4Most);
       }
     }
 #pragma unroll
     for (int span = 1; span < kWords; span *= 2) {
       if (group <= 32 * span) break;
 #pragma unroll
-      for (int i = 0; i < kWords; i += 2 * span) {
-        lo[i] = fminf(lo[i], lo[i + span]), hi[i] = fmaxf(hi[i], hi[i + span]), nan[i] += nan[i + span];
-      }
+      for (int i = 0; i < kWords; i += 2 * span) lo[i] = fminf(lo[i], lo[i + span]), hi[i] = max_nan(hi[i], hi[i + span]);
     }
-    const int step_words = group / 32;
+    const int step_log2 = group_log2 - 5;
     float off = 0.0f, inv = 0.0f;
     bool any = false;
     __half scale_h = __float2half_rn(0.0f), offset_h = scale_h;
 #pragma unroll
     for (int i = 0; i < kWords; ++i) {
-      if (i % step_words == 0) {  // a group begins: its parameters
+      if ((i & ((1 << step_log2) - 1)) == 0) {  // a group begins: its parameters
 #pragma unroll
         for (int o = 1; o < 4; o <<= 1) {
           lo[i] = fminf(lo[i], __shfl_xor_sync(0xffffffffu, lo[i], o));
-          hi[i] = fmaxf(hi[i], __shfl_xor_sync(0xffffffffu, hi[i], o));
-          nan[i] += __shfl_xor_sync(0xffffffffu, nan[i], o);
+          hi[i] = max_nan(hi[i], __shfl_xor_sync(0xffffffffu, hi[i], o));
         }
-        scale_h = __float2half_rn(__fadd_rn(__fdiv_rn(__fsub_rn(hi[i], lo[i]), 15.0f), nan[i]));
+        const float low = fminf(fmaxf(lo[i], -kKv4Most), kKv4Most);
+        const float high = hi[i] != hi[i] ? hi[i] : fminf(fmaxf(hi[i], -kKv4Most), kKv4Most);
+        scale_h = __float2half_rn(fifteenth(__fsub_rn(high, low)));
         const float s = __half2float(scale_h);
-        offset_h = __float2half_rn(__fadd_rn(lo[i], __fmul_rn(8.0f, s)));
+        offset_h = __float2half_rn(__fadd_rn(low, __fmul_rn(8.0f, s)));
         off = __half2float(offset_h);
         any = s > 0.0f;
-        inv = any ? __fdiv_rn(1.0f, s) : 0.0f;
+        inv = any ? __frcp_rn(s) : 0.0f;
         if (t == 0 && to.tile)
-          reinterpret_cast<uint32_t *>(to.tile + 16 * D + (is_v ? 64 * ng : 0))[to.tok * ng + i / step_words] =
+          reinterpret_cast<uint32_t *>(to.tile + 16 * D + (is_v ? 64 * ng : 0))[to.tok * ng + (i >> step_log2)] =
               (uint32_t)__half_as_ushort(scale_h) | (uint32_t)__half_as_ushort(offset_h) << 16;
       }
       uint32_t w = 0;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float y = any ? rintf(__fmul_rn(__fsub_rn(x[i][e], off), inv)) : 0.0f;
-        const uint32_t code = (uint32_t)((int)fminf(fmaxf(y, -8.0f), 7.0f) + 8);
+        // to the nearest integer, ties to even, by adding 1.5 * 2^23 (and the 8): it is then
+        // in the low bits; conversions would go through the unit with 16 results a cycle
+        const float y = any ? fminf(fmaxf(__fmul_rn(__fsub_rn(x[i][e], off), inv), -8.0f), 7.0f) : 0.0f;
+        const uint32_t code = __float_as_uint(__fadd_rn(y, 12582920.0f)) & 15u;
         w |= code << (4 * (is_v ? e : (e & 1) * 4 + e / 2));
       }
       words[i] = w;
@@ -480,17 +494,17 @@ __global__ void __launch_bounds__(kTokenThreads)
 
 template <typename T, int D>
 __global__ void __launch_bounds__(kTokenThreads)
-    kv4_read_kernel(const Kv4View c, const int group, T *__restrict__ k, T *__restrict__ v, const bool vec,
+    kv4_read_kernel(const Kv4View c, const int group_log2, T *__restrict__ k, T *__restrict__ v, const bool vec,
                     const int64_t *__restrict__ slots, const int n) {
   constexpr int kSlabs = D > 128 ? 2 : 1, kWpr = D / kSlabs / 32, kWords = D / 32;
-  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3, ng = D / group;
-  const int64_t id = (int64_t)blockIdx.x * (kTokenThreads / 32) + (threadIdx.x >> 5);
-  const int head = (int)(id % c.kv_heads);
-  const bool is_v = id / c.kv_heads & 1;
-  const int64_t first = id / c.kv_heads / 2 * kTokensWarp;
+  const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+  const int ng = D >> group_log2;
+  const uint32_t id = blockIdx.x * (kTokenThreads / 32) + (threadIdx.x >> 5), part = id / (uint32_t)c.kv_heads;
+  const int head = (int)(id - part * c.kv_heads);
+  const bool is_v = part & 1;
+  const int64_t first = (int64_t)(part >> 1) * kTokensWarp;
   if (first >= n) return;
-  const Spot mine = load_spot(c, slots, n, first, head, kv4_tile_bytes(D, group));
-  const int step_words = group / 32;
+  const Spot mine = load_spot(c, slots, n, first, head, 16 * D + 128 * ng);
   {
     const Spot at = spot_of(mine, g);
     uint32_t w[kWords], par[kWords];
@@ -499,7 +513,7 @@ __global__ void __launch_bounds__(kTokenThreads)
     if (at.tile) {
       const uint32_t *params = reinterpret_cast<const uint32_t *>(at.tile + 16 * D + (is_v ? 64 * ng : 0)) + at.tok * ng;
 #pragma unroll
-      for (int i = 0; i < kWords; ++i) par[i] = params[i / step_words];
+      for (int i = 0; i < kWords; ++i) par[i] = params[i >> (group_log2 - 5)];
     }
     if (!is_v) {
       if (at.tile) {
@@ -523,14 +537,15 @@ __global__ void __launch_bounds__(kTokenThreads)
       const uint32_t pick = (s0.tok & 1 ? 0x32u : 0x10u) | (s1.tok & 1 ? 0x7600u : 0x5400u);
 #pragma unroll
       for (int i = 0; i < kWords; ++i) {
-        const uint32_t both = __byte_perm(a[i], b[i], pick);  // 4 nibbles (dims 8 apart) of each token
-        // lane (row, t) wants, of its row, nibble t of dims 0 .. 7: they are with the lanes
-        // (dim, row / 2), in the half row % 2
-        uint32_t y = 0;
+        // 4 nibbles (dims 8 apart) of each token: as 16-bit elements an 8 x 8 matrix, dims by
+        // tokens. Transposed, a lane has dims 2 t and 2 t + 1 of its own token, and wants
+        // nibble t of all eight, which are with the four lanes of the token.
+        uint32_t both = __byte_perm(a[i], b[i], pick), y = 0;
+        asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %0;" : "+r"(both));
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          const uint32_t x = __shfl_sync(0xffffffffu, both, e * 4 + g / 2);
-          y |= (x >> (16 * (g & 1) + 4 * t) & 15u) << (4 * e);
+        for (int q = 0; q < 4; ++q) {
+          const uint32_t x = __shfl_sync(0xffffffffu, both, (lane & 28) + q) >> (4 * t);
+          y |= ((x & 15u) | (x >> 12 & 0xf0u)) << (8 * q);
         }
         w[i] = y;
       }
@@ -565,7 +580,7 @@ cudaError_t launch_append(const Kv4View &c, int group, const void *k, const void
   const bool vec = ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) == 0 &&
                    ((st.k_token | st.k_head | st.v_token | st.v_head) & (int64_t)(unit - 1)) == 0;
   kv4_append_kernel<T, D><<<(unsigned)token_blocks(c, n), kTokenThreads, 0, stream>>>(
-      c, group, static_cast<const T *>(k), static_cast<const T *>(v), st, vec, slots, n);
+      c, 31 - __builtin_clz((unsigned)group), static_cast<const T *>(k), static_cast<const T *>(v), st, vec, slots, n);
   return cudaGetLastError();
 }
 
@@ -574,7 +589,7 @@ cudaError_t launch_read(const Kv4View &c, int group, void *k, void *v, const int
                         cudaStream_t stream) {
   const bool vec = ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) == 0;
   kv4_read_kernel<T, D><<<(unsigned)token_blocks(c, n), kTokenThreads, 0, stream>>>(
-      c, group, static_cast<T *>(k), static_cast<T *>(v), vec, slots, n);
+      c, 31 - __builtin_clz((unsigned)group), static_cast<T *>(k), static_cast<T *>(v), vec, slots, n);
   return cudaGetLastError();
 }
 
@@ -591,8 +606,8 @@ cudaError_t by_form(int dtype, int d, F f) {
   return with(float{});
 }
 
-// The last grid index of a launch over n tokens has to stay inside 31 bits.
-bool tokens_fit(const Kv4View &c, int32_t n) { return token_blocks(c, n) < 0x7fffffffull; }
+// The warps of a launch over n tokens are counted in 31 bits.
+bool tokens_fit(const Kv4View &c, int32_t n) { return token_blocks(c, n) * (kTokenThreads / 32) < 0x7fffffffull; }
 
 }  // namespace
 

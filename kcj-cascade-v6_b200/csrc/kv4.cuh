@@ -54,9 +54,9 @@ CB_D float kv4_scale(uint32_t par) { return __half2float(__ushort_as_half((unsig
 CB_D float kv4_offset(uint32_t par) { return __half2float(__ushort_as_half((unsigned short)(par >> 16))); }
 
 // The value of a code. scale * (code - 8) is exact in fp32 (11 + 4 bits), so the
-// fused form rounds once, as the separate one does.
+// fused form rounds once, as the separate one does. (2^23 | code is 2^23 + code.)
 CB_D float kv4_value(uint32_t code, float scale, float offset) {
-  return fmaf(scale, (float)((int)code - 8), offset);
+  return fmaf(scale, __uint_as_float(0x4b000000u | code) - 8388616.0f, offset);
 }
 
 template <typename T>
