@@ -791,17 +791,21 @@ auto by_form(int d, int ng, int nt, F f) {
   return with_ng(std::integral_constant<int, 256>{});
 }
 
-// Row tiles of 8, 16 or 32 rows: the smallest that holds the rows of a
-// request, so that the cache is read once. Larger ones would leave no
-// registers (O is D*rows/32 of them in a lane), so more rows are more tiles.
+// n-tiles of a row tile (8, 16 or 32 rows) for requests of `rows` rows. A tile of 32
+// rows has room for 8 warps on an SM (O is head_dim * rows / 32 registers in a lane),
+// one of 8 rows for 16, and costs 3.5 times as much; what several tiles read again is
+// in L2. 24 requests of up to 7,000 tokens, 8 KV heads of 128, us with tiles of 8,
+// 16, 32 rows: 16 rows 54, 52, -; 24 rows 74, 87, 79; 32 rows 91, 89, 84; 40
+// rows 111, 126, 133; 64 rows 166, 163, 139.
 int few_tiles(int head_dim, int64_t rows) {
   if (rows <= 8) return 1;
-  return rows <= 16 || head_dim > 128 ? 2 : 4;
+  if (rows <= 16 || head_dim > 128) return 2;
+  return 2 * ((rows + 7) / 8) > 7 * ((rows + 31) / 32) ? 4 : 1;
 }
 
 // Above this many rows of a request the prompt kernel takes it (where it is
 // offered: head_dim 64 and 128). It works on 128 rows whether there are or not, the
-// few-row kernel reads the cache once for every 32. 24 requests of up to 7,000
+// few-row kernel reads the cache again for every 8 or 32. 24 requests of up to 7,000
 // tokens, 8 KV heads of 128, few-row against prompt kernel: 64 rows 139 against 180
 // us, 96 rows 197 against 186, 128 rows 252 against 186.
 constexpr int kFewRows = 64;
