@@ -18,7 +18,8 @@ positions in one launch, without a host round trip.
     plan = table.plan(q_lens, tokens=len(hidden))
     for layer in range(28):
         cache.append(layer, k, v, plan.slots)
-        o = cache.attend(layer, q, table.block_table, table.kv_lens, q_start=plan.q_start)
+        o = cache.attend(layer, q, table.block_table, table.kv_lens, q_start=plan.q_start,
+                         max_q=longest)
 
 All calls run on the current stream of the cache's device, allocate only their
 outputs (and attend a workspace) from torch's allocator, never wait for the

@@ -327,7 +327,13 @@ __global__ void __launch_bounds__(kThreads, Form<D, NG, NT>::kCtasPerSm)
     int since = 0;
 #pragma unroll 1
     for (int tile0 = w.t0; tile0 < w.t1; tile0 += 2) {
-      if (!bar_wait(bars + 8 * half, parity >> half & 1)) kv4_error(c.errors, kErrTimeout);
+      if (!__all_sync(0xffffffffu, bar_wait(bars + 8 * half, parity >> half & 1))) {
+        // The results are void. The other half's copies are given their time to end.
+        kv4_error(c.errors, kErrTimeout);
+        bar_wait(bars + 8 * (half ^ 1), parity >> (half ^ 1) & 1);
+        if (lane == 0) a.join_how[piece] = kJoinNone;
+        return;
+      }
       parity ^= 1u << half;
       const uint32_t there = ok >> (2 * half) & 3u;
       constexpr int J = F::kJoint;
