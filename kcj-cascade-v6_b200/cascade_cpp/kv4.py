@@ -282,7 +282,7 @@ class PageTable:
 
     ``block_table``, ``kv_lens``, ``borrowed`` (leading pages of a row that it
     does not own), ``free`` and ``free_count`` (a stack of page numbers and its
-    height) are plain int32 tensors that a program may also set itself."""
+    height) are plain int32 tensors that a program may also write, in place."""
 
     def __init__(self, requests: int, columns: int, num_pages: int, page_size: int = 16, device=None):
         if requests < 0 or columns <= 0 or num_pages <= 0 or page_size <= 0:
@@ -325,20 +325,24 @@ class PageTable:
         tokens = int(tokens)
         if tokens < 0:
             raise ValueError("tokens must not be negative")
-        if out is None:
+        kv_lens, count = self.kv_lens, self.free_count
+        if out is None:  # the int32 outputs share one allocation
             slots = torch.empty(tokens, dtype=torch.int64, device=dev)
-            positions = torch.empty(tokens, dtype=i32, device=dev)
-            q_start = torch.empty(n + 1, dtype=i32, device=dev)
             status = torch.empty(n, dtype=torch.uint8, device=dev)
+            if commit:
+                positions, q_start = torch.empty(tokens + n + 1, dtype=i32, device=dev).split_with_sizes(
+                    (tokens, n + 1))
+            else:
+                positions, q_start, kv_lens, count = torch.empty(tokens + 2 * n + 2, dtype=i32, device=dev
+                                                                 ).split_with_sizes((tokens, n + 1, n, 1))
         else:
             slots, positions, q_start, status = out[:4]
             _vector(slots, "out.slots", torch.int64, dev, tokens)
             _vector(positions, "out.positions", i32, dev, tokens)
             _vector(q_start, "out.q_start", i32, dev, n + 1)
             _vector(status, "out.status", torch.uint8, dev, n)
-        kv_lens, count = self.kv_lens, self.free_count
-        if not commit:
-            kv_lens, count = torch.empty_like(kv_lens), torch.empty_like(count)
+            if not commit:
+                kv_lens, count = torch.empty_like(kv_lens), torch.empty_like(count)
         a = L.cb_kv4_plan_args(
             lens, done, self.kv_lens.data_ptr(), kv_lens.data_ptr(), self.borrowed.data_ptr(),
             self.block_table.data_ptr(), self.free.data_ptr(), self.free_count.data_ptr(), count.data_ptr(),
