@@ -232,7 +232,7 @@ class KV4Cache(KVPageConnector):
         if start is None and rows != n:
             raise ValueError("without q_start there is one row for each request")
         if out is None:
-            out = torch.empty((rows, heads, d), dtype=q.dtype, device=dev)
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
         elif (not isinstance(out, torch.Tensor) or out.device != dev or out.dtype != q.dtype
               or out.shape != q.shape or not out.is_contiguous() or out.data_ptr() % 16):
             raise ValueError("out must be contiguous, 16-byte aligned and like q")
