@@ -37,7 +37,7 @@ namespace {
 // of K and V. Measured: 48 requests of 9,000 to 32,000 tokens, 64 / 8 heads of 128,
 // group 128: 214 us, 5.0 TB/s; the rest of the way is instructions (266 for a tile
 // of 16 tokens, 16 of them products and 80 the unpacking, at 0.6 an SM quarter and
-// cycle). A single short request is bound by latency: 11.4 us for 1,100 tokens.
+// cycle). A single short request is bound by latency: 10.7 us for 1,100 tokens.
 // mma.sync and not tcgen05: its operands come from registers, where the codes become
 // them with one instruction for two values, and 8 rows leave 15/16 of a 128-row
 // product empty; kv4_prompt.cu has the rows for that.

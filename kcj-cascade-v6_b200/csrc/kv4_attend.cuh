@@ -223,16 +223,13 @@ CB_D long long block_scan(long long v, long long *sums, long long &all) {
   return v;
 }
 
-// Finds the warp's piece [f0, f1) of the line (the block's, if L::kBlock) and the
-// item that holds f0, which begins at `first`; false if there is nothing left for
-// it. Neighbouring pieces are on different SMs, so that a short line is spread
-// over all of them. All threads of the block call; `sums` has two entries for
-// each warp, `ends` one for each thread, in shared memory.
+// find_piece for more requests than a warp has lanes: prefix sums over the block.
 template <typename L>
-CB_D bool find_piece(const AttendArgs &a, const Kv4View &c, int most, long long *sums, long long *ends,
-                     long long &share, long long &f0, long long &f1, long long &first, Item &it) {
+CB_D void find_among_many(const AttendArgs &a, const Kv4View &c, int most, long long *sums, long long *ends, int pieces,
+                          long long place, long long &share, long long &f0, long long &f1, long long &first, Item &it,
+                          bool &found) {
   constexpr int kWarps = L::kWarps, kThreads = kWarps * 32;
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
   long long total = 0, mine = 0;
   for (int b = threadIdx.x; b < a.requests; b += kThreads) {
     mine = request_tiles<L>(a, c.kv_heads, most, b);
@@ -243,11 +240,9 @@ CB_D bool find_piece(const AttendArgs &a, const Kv4View &c, int most, long long 
   const bool once = a.requests <= kThreads;  // a thread has a request at most
   long long chunk, v = block_scan<kWarps>(total, sums, chunk);
   total = chunk;
-  const int pieces = gridDim.x * (L::kBlock ? 1 : kWarps);
   share = max(quotient(total + pieces - 1, pieces), (long long)a.min_share);
-  f0 = (long long)((L::kBlock ? 0 : warp * gridDim.x) + blockIdx.x) * share;
+  f0 = place * share;
   f1 = min(f0 + share, total);
-  bool found = false;
   long long before = 0;
   for (int b0 = 0; b0 < a.requests; b0 += kThreads) {
     if (!once) {
@@ -268,6 +263,44 @@ CB_D bool find_piece(const AttendArgs &a, const Kv4View &c, int most, long long 
     }
     before += chunk;
     if (!once) __syncthreads();
+  }
+}
+
+// Finds the warp's piece [f0, f1) of the line (the block's, if L::kBlock) and the
+// item that holds f0, which begins at `first`; false if there is nothing left for
+// it. Neighbouring pieces are on different SMs, so that a short line is spread
+// over all of them. All threads of the block call; `sums` has two entries for
+// each warp, `ends` one for each thread, in shared memory.
+template <typename L>
+CB_D bool find_piece(const AttendArgs &a, const Kv4View &c, int most, long long *sums, long long *ends,
+                     long long &share, long long &f0, long long &f1, long long &first, Item &it) {
+  constexpr int kWarps = L::kWarps;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int pieces = gridDim.x * (L::kBlock ? 1 : kWarps);
+  const long long place = (L::kBlock ? 0 : warp * gridDim.x) + blockIdx.x;
+  bool found = false;
+  if (a.requests <= 32) {  // every warp for itself, a lane to a request: no barriers
+    long long v = 0;
+    if (lane < a.requests) {
+      v = request_tiles<L>(a, c.kv_heads, most, lane);
+      const int len = __ldg(a.kv_lens + lane);
+      if (blockIdx.x == 0 && warp == 0 && (len < 0 || len > most)) kv4_error(c.errors, kErrBounds);
+    }
+    for (int o = 1; o < a.requests; o <<= 1) {
+      const long long y = __shfl_up_sync(0xffffffffu, v, o);
+      if (lane >= o) v += y;
+    }
+    const long long total = __shfl_sync(0xffffffffu, v, a.requests - 1);
+    share = max(quotient(total + pieces - 1, pieces), (long long)a.min_share);
+    f0 = place * share;
+    f1 = min(f0 + share, total);
+    const int n = __popc(__ballot_sync(0xffffffffu, lane < a.requests && v <= f0));
+    it.b = n;
+    first = __shfl_sync(0xffffffffu, v, max(n - 1, 0));
+    if (n == 0) first = 0;
+    found = f0 < total;
+  } else {
+    find_among_many<L>(a, c, most, sums, ends, pieces, place, share, f0, f1, first, it, found);
   }
   if (!found || f0 >= f1) return false;
   load_request(a, most, it.b, it.q0, it.qn, it.len);
