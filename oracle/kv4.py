@@ -141,6 +141,90 @@ def attend(q, k, v, kv_len, causal, scale):
     return out, lse, slack
 
 
+def params(pages: Pages, layer, slots):
+    """float64 (scale, offset) of K and of V, each [n, heads, dim]."""
+    ng = pages.dim // pages.group
+    out = []
+    for par_at in (16 * pages.dim, 16 * pages.dim + 64 * ng):
+        par = np.zeros((len(slots), pages.data.shape[2], ng, 2))
+        for n, slot in enumerate(slots):
+            tile, tok = pages._tile(layer, slot)
+            a = par_at + tok * ng * 4
+            par[n] = np.ascontiguousarray(tile[:, a:a + 4 * ng]).view(np.float16).reshape(-1, ng, 2)
+        out.append(tuple(np.repeat(par[..., i], pages.group, 2) for i in (0, 1)))
+    return out
+
+
+# Roundings of distinct values are taken as independent and of either sign: a sum of
+# them, each at most a_t, passes 7.5 * sqrt(sum a_t^2) once in 10^12 (Hoeffding).
+SIGMAS = 7.5
+
+
+def attend_bounds(q, k, v, kv_len, causal, scale, par=None):
+    """One request, as attend() -> (out, lse, tol_out [n, heads, dim], tol_lse [n, heads]):
+    how far a kernel may be off before its output is rounded to its type.
+
+    With ``par`` (params() of its tokens) for the kernel of few rows, which multiplies
+    raw codes (exact in fp16) and rounds only p * scale_v to fp16; without, for the kernel
+    of many rows, whose K, V and p are fp16. e(x) below is 2^-x.
+
+    Sums of products are in 32 bits, with low bits cut off: a step of 16 terms costs
+    e(22) of the largest value that the running sum takes. A score: dim / 16 steps of
+    up to sum |q| * 15 scale (codes) or sum |q k|; the kernel of few rows also takes sum(q) (dim / 8
+    + 4 additions of e(24)) times offset - 8 scale. Its exponential: the argument to e(24)
+    relative, the result to e(22). The sum of weights: kv_len / 8 additions of e(24).
+    Outputs: kv_len / 16 steps on the running sum; codes are uncentred, 15 scale each, for 8
+    tiles of 16 tokens at a time.
+    A weight below 2^-14 of the largest, in fp16: e(25) of the largest."""
+    n, heads, dim = q.shape
+    ratio = heads // k.shape[1]
+    few = par is not None
+    e = lambda x: 2.0 ** -x  # noqa: E731
+    out, lse = np.zeros((n, heads, dim)), np.full((n, heads), -np.inf)
+    tol, tol_l = np.zeros((n, heads, dim)), np.zeros((n, heads))
+    for r in range(n):
+        limit = kv_len - (n - 1 - r) if causal else kv_len
+        if limit <= 0:
+            continue
+        for h in range(heads):
+            j = h // ratio
+            kk, vv, qq = k[:limit, j], v[:limit, j], q[r, h]
+            s = kk @ qq * scale
+            p = np.exp(s - s.max())
+            total = p.sum()
+            lse[r, h] = s.max() + np.log(total)
+            p /= total
+            o = p @ vv
+            out[r, h] = o
+            a, extra, extra_l = np.abs(qq), 0.0, 0.0
+            if few:
+                (ks, ko), (vs, vo) = [tuple(x[:limit, j] for x in both) for both in par]
+                w = ((dim / 16 + 1) * e(22) * (15 * ks @ a)
+                     + ((dim / 8 + 4) * e(24) + e(22)) * ((np.abs(ko) + 8 * ks) @ a)) * abs(scale)
+                c = vv - vo  # scale * (code - 8)
+                round_p = SIGMAS * e(11) * np.sqrt(((p[:, None] * c) ** 2).sum(0))
+                round_p += limit * e(22) * (p[:, None] * vs).max()  # weights that are subnormal
+                steps = 8 * e(22) * 15 * (p[:, None] * vs).sum(0) * 2
+                steps += (limit / 16 + 1) * e(22) * np.abs(np.cumsum(p[:, None] * c, 0)).max(0)
+                steps += (limit / 8 + 16) * e(24) * (p[:, None] * np.abs(vo)).sum(0)
+            else:
+                k16, v16 = kk.astype(np.float16).astype(np.float64), vv.astype(np.float16).astype(np.float64)
+                s16 = k16 @ qq * scale
+                p16 = np.exp(s16 - s16.max())
+                extra_l = np.abs(s16.max() + np.log(p16.sum()) - lse[r, h])
+                p16 /= p16.sum()
+                extra = np.abs(p16 @ v16 - o)
+                w = (dim / 16 + 2) * e(22) * (np.abs(kk) @ a) * abs(scale)
+                round_p = SIGMAS * e(11) * np.sqrt(((p[:, None] * vv) ** 2).sum(0))
+                round_p += limit * e(25) * p.max() * np.abs(vv).max(0)
+                steps = (limit / 16 + 1) * e(22) * np.abs(np.cumsum(p[:, None] * vv, 0)).max(0)
+            w = np.expm1(w + e(22) + e(23) * (1 + np.abs(s).max()))
+            sums = (limit / 8 + 16) * e(24)
+            tol[r, h] = (p * w) @ np.abs(vv - o) * 2 + round_p + steps + sums * np.abs(o) + extra
+            tol_l[r, h] = (p * w).sum() * 2 + sums + e(22) * (1 + np.abs(lse[r, h])) + extra_l
+    return out, lse, tol, tol_l
+
+
 class Table:
     """PageTable.plan, row by row."""
 
