@@ -70,6 +70,7 @@ struct Form {
   static constexpr int kConst = kRows * (2 + NG) * 4;
   static constexpr int kWarp = (kRing + kQ + kConst + 16 + 127) / 128 * 128;
   static constexpr int kSmem = kWarps * kWarp;
+  static constexpr int kStatic = (2 * kWarps + kThreads) * (int)sizeof(long long);  // of find_piece
   static constexpr int kPart = kRows * (D + 2);     // floats of a partial result
   struct Line {
     static constexpr int kRows = 8 * NT, kTokens = kKv4Tile, kCost = kItemCost, kWarps = cb::kWarps;
@@ -760,6 +761,7 @@ template <int D, int NG, int NT>
 cudaError_t run_few(const Kv4View &c, const AttendArgs &a, const Launch &l, cudaStream_t stream) {
   using F = Form<D, NG, NT>;
   static std::atomic<uint64_t> ready{0};  // a bit for each device
+  static_assert(F::kCtasPerSm * (F::kSmem + F::kStatic + 1024) <= 228 * 1024, "shared memory of an SM");
   cudaError_t e = allow_shared(attend_few_kernel<D, NG, NT>, F::kSmem, ready);
   if (e != cudaSuccess) return e;
   attend_few_kernel<D, NG, NT><<<l.pieces / kWarps, kThreads, F::kSmem, stream>>>(c, a);
@@ -776,14 +778,18 @@ cudaError_t run_few(const Kv4View &c, const AttendArgs &a, const Launch &l, cuda
   return cudaLaunchKernelEx(&cfg, attend_join_kernel<D>, a, l.pieces, NT);
 }
 
+// n-tiles of a row tile at most: O is head_dim * rows / 32 registers of a lane, and 8
+// warps' rings and query rows have to fit an SM (256 dims in 8 groups, 16 rows: 230 KB).
+constexpr int most_tiles(int d, int ng) { return d <= 128 ? 4 : ng <= 4 ? 2 : 1; }
+
 // f(integral constants D, NG, NT) for a cache and a number of n-tiles.
 template <typename F>
 auto by_form(int d, int ng, int nt, F f) {
   auto with_nt = [&](auto dd, auto gg) {
-    constexpr int kD = decltype(dd)::value;
+    constexpr int kMost = most_tiles(decltype(dd)::value, decltype(gg)::value);
     if (nt == 1) return f(dd, gg, std::integral_constant<int, 1>{});
-    if (nt == 2 || kD > 128) return f(dd, gg, std::integral_constant<int, 2>{});
-    return f(dd, gg, std::integral_constant<int, (kD > 128 ? 2 : 4)>{});
+    if (nt == 2) return f(dd, gg, std::integral_constant<int, (kMost < 2 ? kMost : 2)>{});
+    return f(dd, gg, std::integral_constant<int, kMost>{});
   };
   auto with_ng = [&](auto dd) {
     constexpr int kD = decltype(dd)::value;
@@ -803,9 +809,10 @@ auto by_form(int d, int ng, int nt, F f) {
 // in L2. 24 requests of up to 7,000 tokens, 8 KV heads of 128, us with tiles of 8,
 // 16, 32 rows: 16 rows 54, 52, -; 24 rows 74, 87, 79; 32 rows 91, 89, 84; 40
 // rows 111, 126, 133; 64 rows 166, 163, 139.
-int few_tiles(int head_dim, int64_t rows) {
-  if (rows <= 8) return 1;
-  if (rows <= 16 || head_dim > 128) return 2;
+int few_tiles(int head_dim, int group, int64_t rows) {
+  const int most = most_tiles(head_dim, head_dim / group);
+  if (rows <= 8 || most == 1) return 1;
+  if (rows <= 16 || most == 2) return 2;
   return 2 * ((rows + 7) / 8) > 7 * ((rows + 31) / 32) ? 4 : 1;
 }
 
@@ -827,7 +834,7 @@ Launches plan_launches(const cb_kv4_cache *cache, const cb_kv4_attend_args *a) {
   Launches l = {};
   l.prompts = d <= 128 && rows > kFewRows;
   // beside prompt chunks the others are single tokens in the main
-  const int nt = few_tiles(d, l.prompts ? ratio : rows);
+  const int nt = few_tiles(d, cache->group, l.prompts ? ratio : rows);
   l.few.sms = min(sm_count(cache->device) & ~1, kJoinThreads);  // a thread of the join counts 16 pieces
   l.few.rows = 8 * nt;
   l.few.part = l.few.rows * (d + 2);

@@ -8,7 +8,7 @@ from cascade_cpp import _lib as L
 from oracle import kv4 as O
 from test_gpu_kv4 import DEV, TYPES, make, nums, tables
 
-DIMS = [(64, 32), (64, 64), (128, 32), (128, 64), (128, 128), (256, 64), (256, 128), (256, 256)]
+DIMS = [(64, 32), (64, 64), (128, 32), (128, 64), (128, 128), (256, 32), (256, 64), (256, 128), (256, 256)]
 
 
 def row_tile(dim, group, rows):

@@ -22,6 +22,11 @@ def test_every_row_tile_with_several_tokens(dim, group):
                   max_q=most)
 
 
+@pytest.mark.parametrize("ratio,qs", [(16, [1, 1]), (7, [2, 3]), (1, [90, 9])])
+def test_dims_256_in_groups_of_32_and_more_rows_than_8(ratio, qs):
+    held_call("bf16", 256, 32, 16, 2, ratio, [140, 60], qs, seed=ratio)
+
+
 @pytest.mark.parametrize("dim,group", [f for f in DIMS if f[0] < 256])
 def test_prompt_chunks_of_every_form(dim, group):
     held_call("fp16", dim, group, 16, 2, 1, [300, 70, 133], [140, 70, 1], seed=dim + group)
