@@ -15,6 +15,7 @@ namespace cb {
 extern thread_local std::string g_create_error;  // store.cu: message of store-less calls
 
 int kv4_fail(int code, const char *msg, cudaError_t e) {
+  if (e != cudaSuccess) (void)cudaGetLastError();  // reported here, and not again by the next launch
   try {
     g_create_error = msg;
     if (e != cudaSuccess) {
@@ -579,18 +580,17 @@ cudaError_t launch_append(const Kv4View &c, int group, const void *k, const void
   const uint64_t unit = 16 / sizeof(T);
   const bool vec = ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) == 0 &&
                    ((st.k_token | st.k_head | st.v_token | st.v_head) & (int64_t)(unit - 1)) == 0;
-  kv4_append_kernel<T, D><<<(unsigned)token_blocks(c, n), kTokenThreads, 0, stream>>>(
-      c, 31 - __builtin_clz((unsigned)group), static_cast<const T *>(k), static_cast<const T *>(v), st, vec, slots, n);
-  return cudaGetLastError();
+  return kv4_launch(kv4_append_kernel<T, D>, dim3((unsigned)token_blocks(c, n)), kTokenThreads, 0, stream, false, c,
+                    31 - __builtin_clz((unsigned)group), static_cast<const T *>(k), static_cast<const T *>(v), st, vec,
+                    slots, n);
 }
 
 template <typename T, int D>
 cudaError_t launch_read(const Kv4View &c, int group, void *k, void *v, const int64_t *slots, int n,
                         cudaStream_t stream) {
   const bool vec = ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) & 15) == 0;
-  kv4_read_kernel<T, D><<<(unsigned)token_blocks(c, n), kTokenThreads, 0, stream>>>(
-      c, 31 - __builtin_clz((unsigned)group), static_cast<T *>(k), static_cast<T *>(v), vec, slots, n);
-  return cudaGetLastError();
+  return kv4_launch(kv4_read_kernel<T, D>, dim3((unsigned)token_blocks(c, n)), kTokenThreads, 0, stream, false, c,
+                    31 - __builtin_clz((unsigned)group), static_cast<T *>(k), static_cast<T *>(v), vec, slots, n);
 }
 
 // f(T{}, std::integral_constant<int, D>{}) for the cache's type and head size.

@@ -81,6 +81,24 @@ CB_D __nv_bfloat16 kv4_round(float x) { return __float2bfloat16_rn(x); }
 int kv4_fail(int code, const char *msg, cudaError_t e = cudaSuccess);
 int kv4_check_cache(const cb_kv4_cache *c, int32_t layer, const char *who, Kv4View *out);
 
+// Launches a kernel and says how that launch went, whatever failed before it. `early`:
+// it may begin before the kernel in front of it has ended, and waits for it itself.
+template <typename... P, typename... A>
+cudaError_t kv4_launch(void (*kernel)(P...), dim3 grid, int threads, size_t shared, cudaStream_t stream, bool early,
+                       A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = shared;
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = early ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<P>(args)...);
+}
+
 // Makes `device` current for the life of the object.
 struct Kv4Device {
   int prev = -1, want;

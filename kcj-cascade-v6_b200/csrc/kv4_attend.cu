@@ -764,18 +764,9 @@ cudaError_t run_few(const Kv4View &c, const AttendArgs &a, const Launch &l, cuda
   static_assert(F::kCtasPerSm * (F::kSmem + F::kStatic + 1024) <= 228 * 1024, "shared memory of an SM");
   cudaError_t e = allow_shared(attend_few_kernel<D, NG, NT>, F::kSmem, ready);
   if (e != cudaSuccess) return e;
-  attend_few_kernel<D, NG, NT><<<l.pieces / kWarps, kThreads, F::kSmem, stream>>>(c, a);
-  if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(8 * l.sms);
-  cfg.blockDim = dim3(kJoinThreads);
-  cfg.stream = stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, attend_join_kernel<D>, a, l.pieces, NT);
+  e = kv4_launch(attend_few_kernel<D, NG, NT>, dim3(l.pieces / kWarps), kThreads, F::kSmem, stream, false, c, a);
+  if (e != cudaSuccess) return e;
+  return kv4_launch(attend_join_kernel<D>, dim3(8 * l.sms), kJoinThreads, 0, stream, true, a, l.pieces, NT);
 }
 
 // n-tiles of a row tile at most: O is head_dim * rows / 32 registers of a lane, and 8

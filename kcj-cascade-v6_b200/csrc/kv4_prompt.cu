@@ -749,18 +749,9 @@ cudaError_t launch(const Kv4View &c, const AttendArgs &a, const Launch &l, cudaS
   static std::atomic<uint64_t> ready{0};  // a bit for each device
   cudaError_t e = allow_shared(attend_prompt_kernel<D, NG>, F::kSmem, ready);
   if (e != cudaSuccess) return e;
-  attend_prompt_kernel<D, NG><<<l.pieces, kPromptThreads, F::kSmem, stream>>>(c, a);
-  if ((e = cudaGetLastError()) != cudaSuccess) return e;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(l.pieces, PromptLine::kRows / 32);
-  cfg.blockDim = dim3(256);
-  cfg.stream = stream;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, prompt_join_kernel<D>, a);
+  e = kv4_launch(attend_prompt_kernel<D, NG>, dim3(l.pieces), kPromptThreads, F::kSmem, stream, false, c, a);
+  if (e != cudaSuccess) return e;
+  return kv4_launch(prompt_join_kernel<D>, dim3(l.pieces, PromptLine::kRows / 32), 256, 0, stream, true, a);
 }
 
 }  // namespace
