@@ -249,7 +249,9 @@ class KV4Cache(KVPageConnector):
         if need is None:
             if len(self._work) > 255:
                 self._work.clear()
-            need = self._work[heads, a.max_q] = lib.cb_kv4_attend_workspace(self._form, a)
+            need = lib.cb_kv4_attend_workspace(self._form, a)
+            if need:  # 0: the call below says what is wrong with its arguments
+                self._work[heads, a.max_q] = need
         work = torch.empty(need, dtype=torch.uint8, device=dev)
         a.workspace, a.workspace_bytes = work.data_ptr(), need
         _check(lib.cb_kv4_attend(self._form, a, _stream(dev)))

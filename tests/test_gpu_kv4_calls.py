@@ -11,6 +11,21 @@ pytestmark = pytest.mark.gpu
 from test_gpu_kv4 import DEV, make  # noqa: E402
 
 
+def i32(*x):
+    return torch.tensor(x, dtype=torch.int32, device=DEV)
+
+
+def test_a_refused_call_does_not_break_the_next():
+    cache, _ = make(4, 1, 2, 64, 16, 32, seed=1)
+    table, lens = torch.arange(4, dtype=torch.int32, device=DEV).view(2, 2), i32(20, 31)
+    q = torch.randn(2, 6, 64, device=DEV).half()
+    want = make(4, 1, 2, 64, 16, 32, seed=1)[0].attend(0, q, table, lens)
+    for layer, x in ((1, q), (-1, q), (0, q.float())):
+        with pytest.raises((TypeError, cascade_cpp.CascadeError)):
+            cache.attend(layer, x, table, lens)
+        assert torch.equal(cache.attend(0, q, table, lens), want)
+
+
 def test_a_failed_call_leaves_no_error_behind():
     cache, _ = make(2, 1, 1, 64, 16, 64, seed=1)
     lib = cascade_cpp._native_lib()
