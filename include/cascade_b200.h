@@ -488,7 +488,9 @@ int cb_kv4_read(const cb_kv4_cache *cache, int32_t layer, int32_t dtype, void *k
  * [total_q][q_heads][head_dim] and the tokens 0 .. kv_lens[i] of its pages
  * block_table[i][..]; row r of its n rows sees the tokens below kv_len - (n -
  * 1 - r) when causal, else all of them. q_heads is a multiple of kv_heads. A
- * row that sees nothing gets zeros and lse -inf; one that sees a NaN gets NaN.
+ * row that sees nothing gets zeros and lse -inf. One that sees a K with a NaN
+ * group is NaN, as its lse; one that sees a V with a NaN group is NaN in the
+ * dimensions of that group, whatever the token's weight.
  * columns * page_size is at most 2^30. out: [total_q][q_heads][head_dim] dense,
  * 16-byte aligned, of q's type, not overlapping q; lse (natural log,
  * [total_q][q_heads] fp32) or NULL. Rows behind q_start[requests] are left as they were. max_q is a hint

@@ -203,10 +203,10 @@ class KV4Cache(KVPageConnector):
         ``[requests + 1]``; without it, one row each) and the first
         ``kv_lens[i]`` tokens of its pages ``block_table[i]``. When ``causal``,
         its last row sees every token and each row before it one fewer; a row
-        that sees nothing gets zeros (log-sum-exp -inf), one that sees a NaN
-        NaN. Query heads are in
-        groups of q_heads / kv_heads that share a KV head. ``scale`` defaults
-        to 1 / sqrt(head_dim). ``max_q`` (rows of a request at most) only helps
+        that sees nothing gets zeros (log-sum-exp -inf). A key that is NaN
+        makes the rows that see it NaN, a NaN group of a value its dimensions
+        in them. Query heads are in groups of q_heads / kv_heads that share a
+        KV head. ``scale`` defaults to 1 / sqrt(head_dim). ``max_q`` (rows of a request at most) only helps
         the choice of kernel. Rows behind the last request are left as they
         were in ``out``. With ``return_lse`` also the log-sum-exp of each row's
         scores, ``[total_q, q_heads]`` fp32. There is no backward pass."""

@@ -458,7 +458,8 @@ __global__ void __launch_bounds__(kThreads, Form<D, NG, NT>::kCtasPerSm)
           }
         }
         // p' = p * scale_v stays near 1 if the maximum is taken over s + log2
-        // scale_v (its exponent; a subnormal scale counts as 2^-15)
+        // scale_v (its exponent; a subnormal scale counts as 2^-15). One that is not
+        // finite wraps to 0, or it would cost the other groups' weights their bits.
         float ev[J][2];
 #pragma unroll
         for (int j = 0; j < J; ++j)
@@ -466,8 +467,8 @@ __global__ void __launch_bounds__(kThreads, Form<D, NG, NT>::kCtasPerSm)
           for (int h = 0; h < 2; ++h) {
             uint32_t top = 0;
 #pragma unroll
-            for (int gi = 0; gi < NG; ++gi) top = max(top, vpar[j][h][gi] & 0x7fffu);
-            ev[j][h] = (float)((int)(top >> 10) - 15);
+            for (int gi = 0; gi < NG; ++gi) top = max(top, (vpar[j][h][gi] << 17) + (1u << 27));
+            ev[j][h] = (float)((int)(top >> 27) - 16);
           }
         float high[NT][2];
         bool raise = false;
@@ -525,15 +526,17 @@ __global__ void __launch_bounds__(kThreads, Form<D, NG, NT>::kCtasPerSm)
             for (int n = 0; n < NT; ++n) {
               const float *p = s[j][n];
               float p0 = p[0] * s0, p1 = p[1] * s0, p2 = p[2] * s1, p3 = p[3] * s1;
-              if (partial) {  // a weight of 0 beside an infinite or NaN scale is nothing
-                if (p[0] == 0.0f) p0 = 0.0f;
-                if (p[1] == 0.0f) p1 = 0.0f;
-                if (p[2] == 0.0f) p2 = 0.0f;
-                if (p[3] == 0.0f) p3 = 0.0f;
-                if (p[0] != 0.0f) z[n][0][gi] = fmaf(p[0], y0, z[n][0][gi]);
-                if (p[1] != 0.0f) z[n][1][gi] = fmaf(p[1], y0, z[n][1][gi]);
-                if (p[2] != 0.0f) z[n][0][gi] = fmaf(p[2], y1, z[n][0][gi]);
-                if (p[3] != 0.0f) z[n][1][gi] = fmaf(p[3], y1, z[n][1][gi]);
+              if (partial) {  // a hidden token's parameters are nothing; a weight of 0 beside a NaN is NaN
+                const int2 lim = *reinterpret_cast<const int2 *>(limits + n * 8 + 2 * t);
+                const int tok = (tile + j) * kKv4Tile + g;
+                if (tok < lim.x) z[n][0][gi] = fmaf(p[0], y0, z[n][0][gi]);
+                else p0 = 0.0f;
+                if (tok < lim.y) z[n][1][gi] = fmaf(p[1], y0, z[n][1][gi]);
+                else p1 = 0.0f;
+                if (tok + 8 < lim.x) z[n][0][gi] = fmaf(p[2], y1, z[n][0][gi]);
+                else p2 = 0.0f;
+                if (tok + 8 < lim.y) z[n][1][gi] = fmaf(p[3], y1, z[n][1][gi]);
+                else p3 = 0.0f;
               } else {
                 z[n][0][gi] = fmaf(p[0], y0, fmaf(p[2], y1, z[n][0][gi]));
                 z[n][1][gi] = fmaf(p[1], y0, fmaf(p[3], y1, z[n][1][gi]));

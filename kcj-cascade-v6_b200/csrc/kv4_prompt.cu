@@ -29,8 +29,9 @@
 // Roundings to 16 bits: K and V as dequantised (2^-11 of a value; the price of one
 // product for a score, where exact codes would need one for every group and two
 // multiplications for every score), P, and the output; q is exact, as in
-// kv4_attend.cu. A V that is NaN or infinite is zero as an operand, or rows that
-// do not see its token would be hurt; rows that do see it (or such a K) become NaN.
+// kv4_attend.cu. A group of V that is not finite is zero as an operand, or rows that
+// do not see its token would be hurt; in rows that do, its dims become NaN (the
+// whole row and its log-sum-exp for such a K), whatever the token's weight.
 #include "kv4_attend.cuh"
 
 namespace cb {
@@ -53,12 +54,13 @@ struct PromptLine {
   static constexpr bool kBlock = true;
 };
 
-struct TileFlags {  // of 128 tokens, written by the dequantising warps
-  uint32_t bad[4];  // a bit for each token whose K or V is not finite
-  uint32_t there;   // two bits in each warp's byte: its cache tiles are there
+struct TileFlags {       // of 128 tokens, written by the dequantising warps
+  uint32_t there;        // in each warp's byte: its two cache tiles are there, and kOdd
   uint32_t pad[3];
+  uint32_t bad_k[4];     // of a warp that set kOdd: a bit for each token whose K is not
+  uint32_t bad_v[4][4];  // finite, and those of V by group
 };
-constexpr uint32_t kAllThere = 0x03030303u;
+constexpr uint32_t kAllThere = 0x03030303u, kOdd = 0x04040404u;
 
 template <int D, int NG>
 struct PromptForm {
@@ -333,15 +335,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
 
         const int limit = row_limit(a, it, min(row, total - 1));
         float l = 0.0f, over = -INFINITY, sub = 0.0f;
+        uint32_t nan_v = 0;  // a bit for each group of which the row sees a V that is not finite
         for (int j = 0; j < n && fine; ++j) {
           fine = warp_wait(bars + 8 * (kScores + x), scores_parity);
           scores_parity ^= 1;
           tc_fence_after();
           const TileFlags &fl = flags[(tile_no + j) & 3];
           const uint32_t there = fl.there;
-          const uint4 bad = *reinterpret_cast<const uint4 *>(fl.bad);
           const int visible = limit - (w.t0 + j) * kTok;  // columns below it are seen
-          const bool masked = __any_sync(0xffffffffu, visible < kTok) || there != kAllThere;
+          const bool masked = __any_sync(0xffffffffu, visible < kTok) || (there & kAllThere) != kAllThere;
           float v[kTok];
 #pragma unroll
           for (int ch = 0; ch < 4; ++ch) tmem_load32(s_at + 32 * ch, v + 32 * ch);
@@ -377,12 +379,15 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
             }
           }
           l *= f;
-          if (bad.x | bad.y | bad.z | bad.w) {
-            const uint32_t b[4] = {bad.x, bad.y, bad.z, bad.w};
-#pragma unroll
+          if (there & kOdd) {
+#pragma unroll 1
             for (int ch = 0; ch < 4; ++ch) {
               const int left = visible - 32 * ch;
-              if (left > 0 && (b[ch] & (left >= 32 ? 0xffffffffu : (1u << left) - 1))) l = NAN;
+              const uint32_t sees = left >= 32 ? 0xffffffffu : left > 0 ? (1u << left) - 1 : 0;
+              if (!(there & kOdd & 0xffu << (8 * ch))) continue;
+              if (fl.bad_k[ch] & sees) l = NAN;
+              for (int gi = 0; gi < NG; ++gi)
+                if (fl.bad_v[gi][ch] & sees) nan_v |= 1u << gi;
             }
           }
           // ---- weights, P over the columns of S
@@ -420,6 +425,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
             float v[32];
             tmem_load32(o_at + d, v);
             tc_wait_ld();
+            if (nan_v >> (d / (D / NG)) & 1) {
+#pragma unroll
+              for (int k = 0; k < 32; ++k) v[k] = NAN;
+            }
             if (!whole) {
 #pragma unroll
               for (int k = 0; k < 8; ++k)
@@ -533,19 +542,26 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
         {  // lane: a token
           const uint32_t *kp = reinterpret_cast<const uint32_t *>(ring + (lane < 16 ? stage : next) * F::kTile + 16 * D) +
                                (lane & 15) * NG;
-          bool bad = false;  // an exponent of all ones in a scale or an offset
+          auto odd = [](uint32_t p) {  // an exponent of all ones in a scale or an offset
+            return (p & 0x7c00) == 0x7c00 || (p >> 16 & 0x7c00) == 0x7c00;
+          };
+          const bool seen = tok0 + lane < sees_most && (there >> (lane >> 4) & 1);
+          bool bad = false;
 #pragma unroll
-          for (int gi = 0; gi < NG; ++gi) {
-            const uint32_t pk = kp[gi], pv = kp[16 * NG + gi];
-            bad |= (pk & 0x7c00) == 0x7c00 || (pk >> 16 & 0x7c00) == 0x7c00;
-            bad |= (pv & 0x7c00) == 0x7c00 || (pv >> 16 & 0x7c00) == 0x7c00;
+          for (int gi = 0; gi < 2 * NG; ++gi) bad |= odd(kp[(gi & 1) * 16 * NG + gi / 2]);
+          const uint32_t votes = __ballot_sync(0xffffffffu, bad && seen);
+          TileFlags &fl = flags[no & 3];
+          if (votes) {
+            bad = false;
+            for (int gi = 0; gi < NG; ++gi) {
+              bad |= odd(kp[gi]);
+              const uint32_t votes_v = __ballot_sync(0xffffffffu, odd(kp[16 * NG + gi]) && seen);
+              if (lane == 0) fl.bad_v[gi][dw] = votes_v;
+            }
+            const uint32_t votes_k = __ballot_sync(0xffffffffu, bad && seen);
+            if (lane == 0) fl.bad_k[dw] = votes_k;
           }
-          bad = bad && tok0 + lane < sees_most && (there >> (lane >> 4) & 1);
-          const uint32_t votes = __ballot_sync(0xffffffffu, bad);
-          if (lane == 0) {
-            flags[no & 3].bad[dw] = votes;
-            reinterpret_cast<uint8_t *>(&flags[no & 3].there)[dw] = (uint8_t)there;
-          }
+          if (lane == 0) reinterpret_cast<uint8_t *>(&fl.there)[dw] = (uint8_t)(there | (votes ? kOdd & 0xffu : 0u));
         }
 #pragma unroll
         for (int ct = 0; ct < 2; ++ct) {

@@ -1,5 +1,6 @@
 """Calls on the paged 4-bit KV cache that are easy to get wrong: after a refused one, with
 values that are not finite, padded, on other streams, on tensors with gradients."""
+import numpy as np
 import pytest
 
 import cascade_cpp
@@ -8,7 +9,8 @@ from cascade_cpp import _lib as L
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
-from test_gpu_kv4 import DEV, make  # noqa: E402
+from kv4_cases import hold  # noqa: E402
+from test_gpu_kv4 import DEV, make, tables  # noqa: E402
 
 
 def i32(*x):
@@ -37,4 +39,55 @@ def test_a_failed_call_leaves_no_error_behind():
     assert lib.cb_kv4_append(cache._form, *call) == L.CB_OK
     assert lib.cb_kv4_append(nowhere, *call) == L.CB_ERR_CUDA
     (x + 1).sum().item()
+
+
+def nan_case(token, far, n=100, group=32, which=1):
+    """One request of 200 tokens and n rows; a group of a token's V (which 1) or K is NaN.
+    ``far``: the token's weight is nothing."""
+    cache, ref = make(14, 1, 1, 128, 16, group, seed=7)
+    table = np.random.default_rng(3).permutation(14)[None, :13].astype(np.int32)
+    kv = [torch.randn(1, 1, 128, device=DEV), torch.randn(1, 1, 128, device=DEV)]
+    if far:
+        kv[0] = torch.full((1, 1, 128), -60.0, device=DEV)
+    kv[which][..., 70] = float("nan")
+    slot = int(table[0, token // 16]) * 16 + token % 16
+    cache.append(0, *kv, torch.tensor([slot], device=DEV))
+    ref.data[:] = cache.cache.cpu().numpy()
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    q = (1.0 + 0.2 * torch.randn(n, 2, 128, generator=gen, device=DEV)).half()
+    return cache, ref, table, q
+
+
+@pytest.mark.parametrize("token", [40, 198])  # in a full tile; in the last one, which two rows see
+@pytest.mark.parametrize("far", [False, True])
+@pytest.mark.parametrize("hint", [1, None])   # the kernel for few rows, and for many
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_a_nan_group_of_v_is_nan_in_its_dims_whatever_its_weight(token, far, hint, group):
+    cache, ref, table, q = nan_case(token, far, group=group)
+    out, lse = cache.attend(0, q, torch.from_numpy(table).to(DEV), i32(200), q_start=i32(0, 100), max_q=hint,
+                            return_lse=True)
+    hold(out, lse, q, ref, 0, table, [200], [100], "fp16", few=hint == 1)
+
+
+@pytest.mark.parametrize("hint", [1, None])
+def test_a_nan_group_of_k_is_nan_in_the_row_and_its_lse(hint):
+    cache, ref, table, q = nan_case(198, False, which=0)
+    out, lse = cache.attend(0, q, torch.from_numpy(table).to(DEV), i32(200), q_start=i32(0, 100), max_q=hint,
+                            return_lse=True)
+    assert torch.isnan(out[-2:]).all() and torch.isnan(lse[-2:]).all()
+    assert torch.isfinite(out[:-2]).all() and torch.isfinite(lse[:-2]).all()
+
+
+@pytest.mark.parametrize("rows,hint", [(1, None), (3, None), (70, None)])
+def test_a_nan_group_of_v_in_one_part_of_a_long_row(rows, hint):
+    cache, ref = make(300, 1, 1, 64, 16, 32, seed=2)
+    table = tables(np.random.default_rng(2), [4700], 300, 16)
+    v = torch.randn(1, 1, 64, device=DEV)
+    v[..., 40] = float("nan")
+    slot = int(table[0, 2000 // 16]) * 16 + 2000 % 16
+    cache.append(0, torch.zeros_like(v), v, torch.tensor([slot], device=DEV))
+    ref.data[:] = cache.cache.cpu().numpy()
+    q = torch.randn(rows, 1, 64, device=DEV).half()
+    out, lse = cache.attend(0, q, torch.from_numpy(table).to(DEV), i32(4700), q_start=i32(0, rows), return_lse=True)
+    hold(out, lse, q, ref, 0, table, [4700], [rows], "fp16")
 
