@@ -421,6 +421,8 @@ int cb_hash_batch_noalloc(int32_t device, const void *const *ptrs, const uint64_
 #define CB_KV4_F32 2
 #define CB_KV4_ERROR_RANGE 1   /* bits of *errors: slot, page or length out of range */
 #define CB_KV4_ERROR_TIMEOUT 2 /* a wait inside a kernel ran out (results are void)  */
+#define CB_KV4_FILL_OUT 1
+#define CB_KV4_FILL_LSE 2
 
 typedef struct cb_kv4_cache {
   void *pages;          /* 16-byte aligned                                   */
@@ -493,8 +495,10 @@ int cb_kv4_read(const cb_kv4_cache *cache, int32_t layer, int32_t dtype, void *k
  * dimensions of that group, whatever the token's weight.
  * columns * page_size is at most 2^30. out: [total_q][q_heads][head_dim] dense,
  * 16-byte aligned, of q's type, not overlapping q; lse (natural log,
- * [total_q][q_heads] fp32) or NULL. Rows behind q_start[requests] are left as they were. max_q is a hint
- * (rows of a request at most); results do not depend on it being right.
+ * [total_q][q_heads] fp32) or NULL. Rows of no request (before q_start[0], behind
+ * q_start[requests]) are left as they were; fill makes them zeros in out
+ * (CB_KV4_FILL_OUT) and -inf in lse (CB_KV4_FILL_LSE). max_q is a hint (rows of a
+ * request at most); results do not depend on it being right.
  * workspace: cb_kv4_attend_workspace bytes, 16-byte aligned, used until the
  * call's work is done. */
 typedef struct cb_kv4_attend_args {
@@ -509,7 +513,7 @@ typedef struct cb_kv4_attend_args {
   int64_t table_stride;
   int64_t q_token_stride, q_head_stride;
   float scale; /* of q.k before the softmax */
-  int32_t layer, dtype, requests, columns, total_q, q_heads, max_q, causal, reserved32;
+  int32_t layer, dtype, requests, columns, total_q, q_heads, max_q, causal, fill;
 } cb_kv4_attend_args;
 int cb_kv4_attend(const cb_kv4_cache *cache, const cb_kv4_attend_args *args, void *stream);
 uint64_t cb_kv4_attend_workspace(const cb_kv4_cache *cache, const cb_kv4_attend_args *args);

@@ -48,6 +48,8 @@ CB_KV4_BF16 = 1
 CB_KV4_F32 = 2
 CB_KV4_ERROR_RANGE = 1
 CB_KV4_ERROR_TIMEOUT = 2
+CB_KV4_FILL_OUT = 1
+CB_KV4_FILL_LSE = 2
 
 
 class cb_config(C.Structure):
@@ -127,7 +129,7 @@ class cb_kv4_attend_args(C.Structure):
         "q", "out", "lse", "block_table", "kv_lens", "q_start", "workspace")] + [
         ("workspace_bytes", C.c_uint64), ("table_stride", C.c_int64), ("q_token_stride", C.c_int64),
         ("q_head_stride", C.c_int64), ("scale", C.c_float)] + [(f, C.c_int32) for f in (
-            "layer", "dtype", "requests", "columns", "total_q", "q_heads", "max_q", "causal", "reserved32")]
+            "layer", "dtype", "requests", "columns", "total_q", "q_heads", "max_q", "causal", "fill")]
 
 
 # (name, restype, argtypes) — exactly the entry points of cascade_b200.h.

@@ -207,9 +207,10 @@ class KV4Cache(KVPageConnector):
         makes the rows that see it NaN, a NaN group of a value its dimensions
         in them. Query heads are in groups of q_heads / kv_heads that share a
         KV head. ``scale`` defaults to 1 / sqrt(head_dim). ``max_q`` (rows of a request at most) only helps
-        the choice of kernel. Rows behind the last request are left as they
-        were in ``out``. With ``return_lse`` also the log-sum-exp of each row's
-        scores, ``[total_q, q_heads]`` fp32. There is no backward pass."""
+        the choice of kernel. Rows of no request (a padded step) are zeros, and
+        left as they were in a given ``out``. With ``return_lse`` also the
+        log-sum-exp of each row's scores, ``[total_q, q_heads]`` fp32, -inf in
+        rows of no request. There is no backward pass."""
         dev, d = self.device, self.head_dim
         _on(q, "q", dev)
         if q.dim() != 3 or q.shape[2] != d or (q.stride(2) != 1 and q.numel()):
@@ -231,8 +232,10 @@ class KV4Cache(KVPageConnector):
         start = None if q_start is None else _vector(q_start, "q_start", torch.int32, dev, n + 1)
         if start is None and rows != n:
             raise ValueError("without q_start there is one row for each request")
+        fill = L.CB_KV4_FILL_LSE if return_lse else 0
         if out is None:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            fill |= L.CB_KV4_FILL_OUT
         elif (not isinstance(out, torch.Tensor) or out.device != dev or out.dtype != q.dtype
               or out.shape != q.shape or not out.is_contiguous() or out.data_ptr() % 16):
             raise ValueError("out must be contiguous, 16-byte aligned and like q")
@@ -243,7 +246,7 @@ class KV4Cache(KVPageConnector):
             q.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(), block_table.data_ptr(), lens,
             start, None, 0, block_table.stride(0), q.stride(0), q.stride(1),
             d ** -0.5 if scale is None else scale, layer, code, n, columns, rows, heads,
-            (1 if start is None else rows) if max_q is None else max_q, causal, 0)
+            (1 if start is None else rows) if max_q is None else max_q, causal, fill)
         lib = _native_lib()
         need = self._work.get((heads, a.max_q))  # the sizes that decide it
         if need is None:

@@ -625,6 +625,22 @@ __global__ void __launch_bounds__(kThreads, Form<D, NG, NT>::kCtasPerSm)
   if (lane == 0) a.join_how[piece] = (uint8_t)how;
 }
 
+// Rows of no request: zeros, and a log-sum-exp of -inf. They are before the first request's
+// rows or behind the last one's.
+template <int D>
+CB_D void fill_rows(const AttendArgs &a) {
+  const int begin = min(max(__ldg(a.q_start), 0), a.total_q);
+  const int end = min(max(__ldg(a.q_start + a.requests), begin), a.total_q);
+  const int64_t rest = (int64_t)(begin + a.total_q - end) * a.q_heads, skip = (int64_t)(end - begin) * a.q_heads;
+  const int64_t from = (int64_t)begin * a.q_heads, step = (int64_t)gridDim.x * kJoinThreads;
+  if (a.fill & CB_KV4_FILL_OUT)
+    for (int64_t i = (int64_t)blockIdx.x * kJoinThreads + threadIdx.x; i < rest * (D / 8); i += step)
+      static_cast<uint4 *>(a.out)[i < from * (D / 8) ? i : i + skip * (D / 8)] = make_uint4(0, 0, 0, 0);
+  if (a.fill & CB_KV4_FILL_LSE)
+    for (int64_t i = (int64_t)blockIdx.x * kJoinThreads + threadIdx.x; i < rest; i += step)
+      a.lse[i < from ? i : i + skip] = -INFINITY;
+}
+
 // Joins the parts of the items that a piece began and did not end, 16 dims of 8
 // rows (a chunk) at a time. A block does eight chunks of an item, a warp each, or
 // one chunk with all its warps where the item has many parts (a long request that
@@ -636,6 +652,8 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const AttendA
   __shared__ float4 tops[kJoinWarps][4];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   const int chunks = nt * (D / 16), groups = (chunks + kJoinWarps - 1) / kJoinWarps;
+  // The kernel in front began after everything before it had ended, and leaves these rows alone.
+  if (a.fill) fill_rows<D>(a);
   asm volatile("griddepcontrol.wait;" ::: "memory");
   // the blocks' tasks, in the order of the pieces; a thread counts 16 pieces
   uint4 how = make_uint4(0, 0, 0, 0);
@@ -854,6 +872,8 @@ int check(const cb_kv4_cache *cache, const cb_kv4_attend_args *a, Kv4View *c) {
     return kv4_fail(CB_ERR_ARG, "cb_kv4_attend: missing array");
   if (reinterpret_cast<uintptr_t>(a->out) & 15)
     return kv4_fail(CB_ERR_ARG, "cb_kv4_attend: out must be 16-byte aligned");
+  if (a->total_q > 0 && (((a->fill & CB_KV4_FILL_OUT) && !a->out) || ((a->fill & CB_KV4_FILL_LSE) && !a->lse)))
+    return kv4_fail(CB_ERR_ARG, "cb_kv4_attend: nothing to fill");
   return CB_OK;
 }
 
@@ -873,11 +893,11 @@ extern "C" int cb_kv4_attend(const cb_kv4_cache *cache, const cb_kv4_attend_args
   using namespace cb;
   Kv4View c;
   if (int rc = check(cache, args, &c)) return rc;
-  if (args->requests == 0 || args->total_q == 0) return CB_OK;
+  if (args->total_q == 0 || (args->requests == 0 && !args->fill)) return CB_OK;
   const Launches l = plan_launches(cache, args);
   const uint64_t need = launch_bytes(l.few) + (l.prompts ? launch_bytes(l.prompt) : 0);
-  if (!args->workspace || args->workspace_bytes < need ||
-      (reinterpret_cast<uintptr_t>(args->workspace) & 15))
+  if (args->requests > 0 &&
+      (!args->workspace || args->workspace_bytes < need || (reinterpret_cast<uintptr_t>(args->workspace) & 15)))
     return kv4_fail(CB_ERR_ARG, "cb_kv4_attend: workspace too small or not 16-byte aligned");
   Kv4Device dev(cache->device);
   if (dev.err != cudaSuccess) return kv4_fail(CB_ERR_CUDA, "cb_kv4_attend: device", dev.err);
@@ -900,8 +920,16 @@ extern "C" int cb_kv4_attend(const cb_kv4_cache *cache, const cb_kv4_attend_args
   a.causal = args->causal;
   a.bf16 = args->dtype == CB_KV4_BF16;
   a.q_vec = ((reinterpret_cast<uintptr_t>(a.q) | (a.q_token_stride | a.q_head_stride) * 2) & 15) == 0;
+  a.fill = args->q_start ? args->fill : 0;  // without q_start every row is a request's
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   cudaError_t e = cudaSuccess;
+  if (args->requests == 0) {
+    const auto join = cache->head_dim == 64    ? attend_join_kernel<64>
+                      : cache->head_dim == 128 ? attend_join_kernel<128>
+                                               : attend_join_kernel<256>;
+    e = kv4_launch(join, dim3(8 * l.few.sms), kJoinThreads, 0, st, false, a, 0, 1);
+    return e == cudaSuccess ? CB_OK : kv4_fail(CB_ERR_CUDA, "cb_kv4_attend: launch", e);
+  }
   if (l.prompts) {
     launch_arrays(l.prompt, static_cast<char *>(args->workspace) + launch_bytes(l.few), a);
     a.rows_above = kFewRows;

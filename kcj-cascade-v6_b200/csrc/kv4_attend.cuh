@@ -39,6 +39,7 @@ struct AttendArgs {
   int32_t requests, columns, total_q, q_heads, ratio, causal, bf16, q_vec;
   int32_t rows_above, rows_most;  // a kernel takes the requests with rows_above < rows <= rows_most
   int32_t min_share;              // of the line, for a piece
+  int32_t fill;                   // CB_KV4_FILL_*
 };
 
 // What an item is: request b, row tile rt, KV head h, and its token tiles.

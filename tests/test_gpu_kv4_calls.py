@@ -91,3 +91,57 @@ def test_a_nan_group_of_v_in_one_part_of_a_long_row(rows, hint):
     out, lse = cache.attend(0, q, torch.from_numpy(table).to(DEV), i32(4700), q_start=i32(0, rows), return_lse=True)
     hold(out, lse, q, ref, 0, table, [4700], [rows], "fp16")
 
+
+@pytest.mark.parametrize("dim,qs", [(64, [3, 7]), (128, [1, 1]), (128, [100, 2]), (256, [20, 1])])
+@pytest.mark.parametrize("first", [0, 2])
+def test_rows_of_no_request_are_zeros_in_a_new_out(dim, qs, first):
+    cache, ref = make(20, 1, 2, dim, 16, 64, seed=4)
+    table, lens = torch.randperm(20, device=DEV).to(torch.int32).view(2, 10), i32(160, 75)
+    start = i32(first, first + qs[0], first + sum(qs))
+    rows = first + sum(qs) + 9
+    q = torch.randn(rows, 4, dim, device=DEV).bfloat16()
+    nan = [torch.full((rows, 4, dim), float("nan"), device=DEV).bfloat16(), torch.full((rows, 4), float("nan"), device=DEV)]
+    del nan  # what the allocator hands out next
+    out, lse = cache.attend(0, q, table, lens, q_start=start, return_lse=True)
+    mine = torch.zeros(rows, dtype=torch.bool, device=DEV)
+    mine[first:first + sum(qs)] = True
+    assert (out[~mine] == 0).all() and torch.isneginf(lse[~mine]).all()
+    hold(out[mine], lse[mine], q[mine], ref, 0, table.cpu().numpy(), [160, 75], qs, "bf16")
+    # a given out keeps them
+    given = torch.full_like(out, 7.0)
+    again, lse = cache.attend(0, q, table, lens, q_start=start, out=given, return_lse=True)
+    assert again is given and (given[~mine] == 7).all() and torch.equal(given[mine], out[mine])
+    assert torch.isneginf(lse[~mine]).all()
+
+
+def test_without_requests_every_row_is_zeros():
+    cache, _ = make(2, 1, 2, 64, 16, 64, seed=4)
+    q = torch.randn(5, 4, 64, device=DEV).half()
+    nan = torch.full_like(q, float("nan"))
+    del nan
+    none = torch.empty(0, dtype=torch.int32, device=DEV)
+    out, lse = cache.attend(0, q, torch.empty(0, 3, dtype=torch.int32, device=DEV), none, q_start=i32(0), return_lse=True)
+    assert (out == 0).all() and torch.isneginf(lse).all()
+
+
+def test_a_padded_step_is_captured_and_replayed():
+    # the number of tokens of a step moves on inside a graph of a fixed token axis
+    cache, _ = make(30, 1, 2, 128, 16, 64, seed=4)
+    table, lens = torch.arange(30, dtype=torch.int32, device=DEV).view(3, 10), i32(90, 150, 31)
+    start = i32(0, 1, 2, 3)
+    q = torch.randn(16, 8, 128, device=DEV).bfloat16()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        cache.attend(0, q, table, lens, q_start=start, max_q=8)
+    torch.cuda.current_stream().wait_stream(s)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = cache.attend(0, q, table, lens, q_start=start, max_q=8)
+    for now in ([0, 8, 12, 16], [0, 1, 2, 3], [0, 0, 0, 1]):
+        start.copy_(i32(*now))
+        g.replay()
+        want = torch.zeros_like(out)
+        cache.attend(0, q, table, lens, q_start=start, max_q=8, out=want)
+        assert torch.equal(out, want) and (out[now[-1]:] == 0).all()
+
