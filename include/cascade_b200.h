@@ -452,7 +452,8 @@ uint64_t cb_kv4_page_bytes(int32_t layers, int32_t kv_heads, int32_t head_dim, i
  * columns * page_size (at most 2^30), or if it needs pages and the rows up to it need more
  * than the stack has; a refused row's pages still count for the rows behind
  * it. Entries behind the last token get slot -1, position 0. kv_lens_out
- * and free_count_out may be kv_lens and free_count. */
+ * and free_count_out may be kv_lens and free_count; block_table gets the new
+ * pages behind those that a row holds in either case. */
 typedef struct cb_kv4_plan_args {
   const int32_t *q_lens;
   const uint8_t *done;   /* or NULL                                          */

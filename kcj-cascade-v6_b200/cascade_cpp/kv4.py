@@ -315,8 +315,10 @@ class PageTable:
         when its tokens end past ``tokens``, do not fit its columns, or need
         pages that are not there; pages are given in row order, and a refused
         row's count against the rows behind it. ``commit=False`` leaves the
-        table as it was (``done`` cannot be given then): the plan says whether
-        the step would fit. ``out`` is an earlier plan of the same ``tokens``
+        lengths and the free pages as they were (``done`` cannot be given
+        then): the plan says whether the step would fit. ``block_table`` names
+        the step's pages behind those that each row holds, where only the
+        plan's own ``kv_lens`` reach. ``out`` is an earlier plan of the same ``tokens``
         whose tensors are written again."""
         n, dev = self.requests, self.device
         i32 = torch.int32

@@ -5,6 +5,7 @@ import pytest
 
 import cascade_cpp
 from cascade_cpp import _lib as L
+from cascade_cpp import kv4
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -145,3 +146,20 @@ def test_a_padded_step_is_captured_and_replayed():
         cache.attend(0, q, table, lens, q_start=start, max_q=8, out=want)
         assert torch.equal(out, want) and (out[now[-1]:] == 0).all()
 
+
+def test_a_dry_plan_names_pages_behind_the_rows_and_changes_nothing_else():
+    t = kv4.PageTable(3, 8, 20, 16, device=DEV)
+    t.plan(i32(20, 0, 33), 53)
+    t.block_table[:, 5:] = -1
+    before = [x.clone() for x in (t.kv_lens, t.borrowed, t.free, t.free_count, t.block_table)]
+    dry = t.plan(i32(40, 3, 0), 50, commit=False)
+    assert all(torch.equal(a, b) for a, b in zip(before, (t.kv_lens, t.borrowed, t.free, t.free_count)))
+    held = [2, 0, 3]
+    for r, n in enumerate(held):
+        assert torch.equal(t.block_table[r, :n], before[4][r, :n])
+    # the plan's slots are in the table, as its program will read them
+    row = torch.tensor([0] * 40 + [1] * 3, device=DEV)
+    pos = dry.positions[:43].long()
+    assert torch.equal(t.block_table[row, pos // 16].long() * 16 + pos % 16, dry.slots[:43])
+    wet = t.plan(i32(40, 3, 0), 50)
+    assert all(torch.equal(a, b) for a, b in zip(dry, wet))
