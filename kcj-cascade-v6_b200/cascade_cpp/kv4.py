@@ -318,8 +318,10 @@ class PageTable:
         lengths and the free pages as they were (``done`` cannot be given
         then): the plan says whether the step would fit. ``block_table`` names
         the step's pages behind those that each row holds, where only the
-        plan's own ``kv_lens`` reach. ``out`` is an earlier plan of the same ``tokens``
-        whose tensors are written again."""
+        plan's own ``kv_lens`` reach. ``out`` is an earlier plan of the same
+        ``tokens`` whose tensors are written again; the lengths and free count
+        of a committed plan are the table's own, which a dry plan does not
+        write."""
         n, dev = self.requests, self.device
         i32 = torch.int32
         lens = _vector(q_lens, "q_lens", i32, dev, n)
@@ -349,7 +351,12 @@ class PageTable:
             _vector(q_start, "out.q_start", i32, dev, n + 1)
             _vector(status, "out.status", torch.uint8, dev, n)
             if not commit:
-                kv_lens, count = torch.empty_like(kv_lens), torch.empty_like(count)
+                kv_lens, count = out[4:]
+                _vector(kv_lens, "out.kv_lens", i32, dev, n)
+                _vector(count, "out.free_count", i32, dev, 1)
+                if count.data_ptr() == self.free_count.data_ptr() or (
+                        n and kv_lens.data_ptr() == self.kv_lens.data_ptr()):
+                    kv_lens, count = torch.empty_like(kv_lens), torch.empty_like(count)
         a = L.cb_kv4_plan_args(
             lens, done, self.kv_lens.data_ptr(), kv_lens.data_ptr(), self.borrowed.data_ptr(),
             self.block_table.data_ptr(), self.free.data_ptr(), self.free_count.data_ptr(), count.data_ptr(),

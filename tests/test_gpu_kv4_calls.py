@@ -163,3 +163,19 @@ def test_a_dry_plan_names_pages_behind_the_rows_and_changes_nothing_else():
     assert torch.equal(t.block_table[row, pos // 16].long() * 16 + pos % 16, dry.slots[:43])
     wet = t.plan(i32(40, 3, 0), 50)
     assert all(torch.equal(a, b) for a, b in zip(dry, wet))
+
+
+def test_a_dry_plan_writes_all_tensors_of_an_earlier_one():
+    t = kv4.PageTable(3, 8, 20, 16, device=DEV)
+    dry = t.plan(i32(20, 0, 33), 53, commit=False)
+    again = t.plan(i32(1, 2, 3), 53, commit=False, out=dry)
+    assert all(a.data_ptr() == b.data_ptr() for a, b in zip(again, dry))
+    assert dry.kv_lens.tolist() == [1, 2, 3] and dry.free_count.item() == 17 and t.kv_lens.tolist() == [0, 0, 0]
+    # a committed plan's lengths are the table's: a dry one never writes those
+    wet = t.plan(i32(1, 2, 3), 53, out=dry)
+    assert wet.kv_lens is t.kv_lens and wet.free_count is t.free_count
+    more = t.plan(i32(5, 5, 5), 53, commit=False, out=wet)
+    assert t.kv_lens.tolist() == [1, 2, 3] and t.free_count.item() == 17
+    assert more.kv_lens.tolist() == [6, 7, 8] and more.slots.data_ptr() == wet.slots.data_ptr()
+    with pytest.raises(ValueError):
+        t.plan(i32(1, 1, 1), 53, commit=False, out=dry._replace(kv_lens=i32(0, 0)))
