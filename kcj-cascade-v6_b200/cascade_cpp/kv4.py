@@ -86,6 +86,17 @@ def _vector(t, name: str, dtype, device, n=None):
     return t.data_ptr()
 
 
+_forward = getattr(getattr(torch, "autograd", None), "forward_ad", None)
+
+
+def _plain(t, name: str):
+    """Refuses a tensor whose gradient or tangent the call would cut off."""
+    if t.requires_grad and torch.is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient, and there is no backward pass: call it under torch.no_grad()")
+    if getattr(_forward, "_current_level", 0) >= 0 and _forward.unpack_dual(t).tangent is not None:
+        raise ValueError(f"{name} has a tangent, and there is no forward-mode derivative")
+
+
 def _dtype_code(dtype) -> int:
     if dtype == torch.bfloat16:
         return L.CB_KV4_BF16
@@ -168,9 +179,11 @@ class KV4Cache(KVPageConnector):
         bits; tokens and heads may be strided, as slices of a fused projection
         are) into ``layer`` of the pages at ``slots`` (int64 ``[n]``, page *
         page_size + offset; negative ones are skipped). A slot may appear once
-        in a call."""
+        in a call. There is no backward pass."""
         self._values(k, "k")
         self._values(v, "v")
+        _plain(k, "k")
+        _plain(v, "v")
         if k.dtype != v.dtype or k.shape[0] != v.shape[0]:
             raise ValueError("k and v differ in type or length")
         n = k.shape[0]
@@ -215,8 +228,7 @@ class KV4Cache(KVPageConnector):
         _on(q, "q", dev)
         if q.dim() != 3 or q.shape[2] != d or (q.stride(2) != 1 and q.numel()):
             raise ValueError(f"q must be [rows, q_heads, {d}] with contiguous heads")
-        if q.requires_grad and torch.is_grad_enabled():
-            raise ValueError("attend has no backward pass: call it under torch.no_grad()")
+        _plain(q, "q")
         rows, heads = q.shape[0], q.shape[1]
         if heads == 0 or heads % self.kv_heads:
             raise ValueError(f"q_heads must be a multiple of {self.kv_heads}")
@@ -239,6 +251,8 @@ class KV4Cache(KVPageConnector):
         elif (not isinstance(out, torch.Tensor) or out.device != dev or out.dtype != q.dtype
               or out.shape != q.shape or not out.is_contiguous() or out.data_ptr() % 16):
             raise ValueError("out must be contiguous, 16-byte aligned and like q")
+        elif out.requires_grad and torch.is_grad_enabled():
+            raise ValueError("out may not require a gradient")
         elif rows and out.data_ptr() == q.data_ptr():
             raise ValueError("out may not be q")
         lse = torch.empty((rows, heads), dtype=torch.float32, device=dev) if return_lse else None

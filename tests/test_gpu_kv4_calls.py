@@ -179,3 +179,28 @@ def test_a_dry_plan_writes_all_tensors_of_an_earlier_one():
     assert more.kv_lens.tolist() == [6, 7, 8] and more.slots.data_ptr() == wet.slots.data_ptr()
     with pytest.raises(ValueError):
         t.plan(i32(1, 1, 1), 53, commit=False, out=dry._replace(kv_lens=i32(0, 0)))
+
+
+def test_tensors_with_gradients_or_tangents_are_refused():
+    cache, ref = make(2, 1, 2, 64, 16, 64, seed=4)
+    table, lens = torch.zeros(3, 1, dtype=torch.int32, device=DEV), i32(3, 4, 5)
+    q, k = torch.randn(3, 4, 64, device=DEV), torch.randn(3, 2, 64, device=DEV)
+    at = torch.arange(3, device=DEV)
+    before = cache.cache.clone()
+    for bad in ((k.clone().requires_grad_(), k), (k, k.clone().requires_grad_())):
+        with pytest.raises(ValueError):
+            cache.append(0, *bad, at)
+    with pytest.raises(ValueError):
+        cache.attend(0, q.half(), table, lens, out=torch.empty_like(q).half().requires_grad_())
+    import torch.autograd.forward_ad as fwd
+    with fwd.dual_level():
+        with pytest.raises(ValueError):
+            cache.append(0, k, fwd.make_dual(k, k), at)
+        with pytest.raises(ValueError):
+            cache.attend(0, fwd.make_dual(q.half(), q.half()), table, lens)
+        cache.attend(0, q.half(), table, lens)
+    assert torch.equal(cache.cache, before)
+    with torch.no_grad():
+        cache.append(0, k.clone().requires_grad_(), k, at)
+        cache.attend(0, q.half().requires_grad_(), table, lens)
+
