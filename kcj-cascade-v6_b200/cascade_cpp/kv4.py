@@ -86,6 +86,25 @@ def _vector(t, name: str, dtype, device, n=None):
     return t.data_ptr()
 
 
+def _overlap(q, out) -> bool:
+    """Whether the dense ``out`` may share memory with ``q [rows, heads, dim]``: it
+    does not where it lies before or behind q, or in a gap between two of its rows."""
+    rows, heads, dim = q.shape
+    if not q.numel():
+        return False
+    size = q.element_size()
+    row, head = q.stride(0), q.stride(1)
+    wide = (heads - 1) * head + dim  # elements that a row spans
+    at = (out.data_ptr() - q.data_ptr()) // size  # of out, from the first of q
+    end = at + -(-out.numel() * out.element_size() // size)
+    if end <= 0 or at >= (rows - 1) * row + wide:
+        return False
+    if rows == 1 or row < wide or at < 0:
+        return True
+    before = at // row  # the last row that begins at or before out
+    return at < before * row + wide or (before + 1 < rows and end > (before + 1) * row)
+
+
 _forward = getattr(getattr(torch, "autograd", None), "forward_ad", None)
 
 
@@ -253,8 +272,8 @@ class KV4Cache(KVPageConnector):
             raise ValueError("out must be contiguous, 16-byte aligned and like q")
         elif out.requires_grad and torch.is_grad_enabled():
             raise ValueError("out may not require a gradient")
-        elif rows and out.data_ptr() == q.data_ptr():
-            raise ValueError("out may not be q")
+        elif _overlap(q, out):
+            raise ValueError("out may not overlap q")
         lse = torch.empty((rows, heads), dtype=torch.float32, device=dev) if return_lse else None
         a = L.cb_kv4_attend_args(
             q.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(), block_table.data_ptr(), lens,

@@ -204,3 +204,13 @@ def test_tensors_with_gradients_or_tangents_are_refused():
         cache.append(0, k.clone().requires_grad_(), k, at)
         cache.attend(0, q.half().requires_grad_(), table, lens)
 
+
+def test_out_may_not_overlap_q():
+    cache, _ = make(4, 1, 2, 64, 16, 64, seed=4)
+    table, lens = torch.zeros(6, 1, dtype=torch.int32, device=DEV), i32(1, 2, 3, 4, 5, 6)
+    raw = torch.randn(7, 4, 64, device=DEV).half()
+    with pytest.raises(ValueError):
+        cache.attend(0, raw[:6], table, lens, out=raw[1:])
+    both = torch.randn(12, 4, 64, device=DEV).half()
+    want = cache.attend(0, both[:6], table, lens)
+    assert torch.equal(cache.attend(0, both[:6], table, lens, out=both[6:]), want)
