@@ -116,6 +116,16 @@ def _plain(t, name: str):
         raise ValueError(f"{name} has a tangent, and there is no forward-mode derivative")
 
 
+def _take_errors(errors) -> int:
+    """The error word, which is 0 again afterwards. The calls may be on any stream."""
+    torch.cuda.synchronize(errors.device)
+    bits = int(errors.item())
+    if bits:
+        errors.zero_()
+        torch.cuda.synchronize(errors.device)  # before a call on another stream sets it
+    return bits
+
+
 def _dtype_code(dtype) -> int:
     if dtype == torch.bfloat16:
         return L.CB_KV4_BF16
@@ -294,11 +304,11 @@ class KV4Cache(KVPageConnector):
         return out if lse is None else (out, lse)
 
     def check(self) -> None:
-        """Waits for the GPU and raises if a call since the last check was given
-        a slot, page or length outside the cache (those are skipped)."""
-        bits = int(self.errors.item())
+        """Waits for the GPU (every stream) and raises if a call since the last
+        check was given a slot, page or length outside the cache (those are
+        skipped)."""
+        bits = _take_errors(self.errors)
         if bits:
-            self.errors.zero_()
             if bits & L.CB_KV4_ERROR_TIMEOUT:
                 raise CascadeError(L.CB_ERR_TIMEOUT, "a wait inside a kernel ran out")
             raise CascadeError(L.CB_ERR_DEVICE, "a slot, page or length was outside the cache")
@@ -441,8 +451,8 @@ class PageTable:
         self.borrowed[row] = n if borrowed else 0
 
     def check(self) -> None:
-        """Waits for the GPU and raises if a plan since the last check met a page
-        or length outside the table (a row that was set wrongly)."""
-        if int(self.errors.item()):
-            self.errors.zero_()
+        """Waits for the GPU (every stream) and raises if a plan since the last
+        check met a page or length outside the table (a row that was set
+        wrongly)."""
+        if _take_errors(self.errors):
             raise CascadeError(L.CB_ERR_DEVICE, "a page or length was outside the table")

@@ -214,3 +214,22 @@ def test_out_may_not_overlap_q():
     both = torch.randn(12, 4, 64, device=DEV).half()
     want = cache.attend(0, both[:6], table, lens)
     assert torch.equal(cache.attend(0, both[:6], table, lens, out=both[6:]), want)
+
+
+def test_check_waits_for_calls_on_every_stream():
+    cache, _ = make(2, 1, 1, 64, 16, 64, seed=4)
+    table = kv4.PageTable(1, 2, 2, 16, device=DEV)
+    x = torch.randn(1, 1, 64, device=DEV).half()
+    at = torch.tensor([777], device=DEV)
+    one, lens = i32(1), i32(-9)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        torch.cuda._sleep(200_000_000)  # about 0.1 s
+        cache.append(0, x, x, at)
+        table.kv_lens.copy_(lens)
+        table.plan(one, 1)
+    with pytest.raises(cascade_cpp.CascadeError):
+        cache.check()
+    with pytest.raises(cascade_cpp.CascadeError):
+        table.check()
