@@ -419,13 +419,16 @@ class PageTable:
         return pages
 
     def give(self, pages: Sequence[int]) -> None:
-        """Puts pages back on the free stack. Waits for the GPU."""
+        """Puts pages back on the free stack, each once. Waits for the GPU."""
         have, n = int(self.free_count.item()), len(pages)
         if n and (min(pages) < 0 or max(pages) >= self.num_pages):
             raise IndexError("page index out of range")
         if have + n > self.num_pages:
             raise CascadeError(L.CB_ERR_ARG, "more pages given back than there are")
-        self.free[have:have + n] = torch.tensor(list(pages), dtype=torch.int32, device=self.device)
+        back = torch.tensor(list(pages), dtype=torch.int32, device=self.device)
+        if len(set(pages)) != n or (n and torch.isin(back, self.free[:have]).any()):
+            raise ValueError("a page is given back twice")
+        self.free[have:have + n] = back
         self.free_count.add_(n)
 
     def attach(self, row: int, pages: Sequence[int], tokens: int, borrowed: bool = False) -> None:
@@ -441,6 +444,8 @@ class PageTable:
             raise ValueError("tokens do not match the pages, or the pages the columns")
         if borrowed and tokens % self.page_size:
             raise ValueError("a borrowed page must be full")
+        if not borrowed and len(set(pages)) != n:
+            raise ValueError("a row owns a page once")
         if n and (min(pages) < 0 or max(pages) >= self.num_pages):
             raise IndexError("page index out of range")
         if int(self.kv_lens[row]):

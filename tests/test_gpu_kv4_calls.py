@@ -181,6 +181,22 @@ def test_a_dry_plan_writes_all_tensors_of_an_earlier_one():
         t.plan(i32(1, 1, 1), 53, commit=False, out=dry._replace(kv_lens=i32(0, 0)))
 
 
+def test_a_page_is_not_given_back_twice():
+    t = kv4.PageTable(2, 4, 6, 16, device=DEV)
+    pages = t.take(3)
+    with pytest.raises(ValueError):
+        t.give([pages[0], pages[0]])
+    t.give(pages[:1])
+    with pytest.raises(ValueError):
+        t.give(pages[:2])  # the first one is free already
+    assert t.free_count.item() == 4
+    t.give(pages[1:])
+    assert sorted(t.free.tolist()) == list(range(6))
+    with pytest.raises(ValueError):
+        t.attach(0, [2, 2], 20)
+    t.attach(0, [2, 2], 32, borrowed=True)
+
+
 def test_tensors_with_gradients_or_tangents_are_refused():
     cache, ref = make(2, 1, 2, 64, 16, 64, seed=4)
     table, lens = torch.zeros(3, 1, dtype=torch.int32, device=DEV), i32(3, 4, 5)
