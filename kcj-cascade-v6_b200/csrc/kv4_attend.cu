@@ -768,14 +768,17 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const AttendA
 constexpr int kMaxDevices = 64;
 
 int sm_count(int device) {
-  static int known[kMaxDevices] = {};
+  static std::atomic<int> known[kMaxDevices];  // calls may come from several threads
   if (device < 0 || device >= kMaxDevices) return 148;
-  if (!known[device]) {
-    int n = 0;
-    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || n <= 0) n = 148;
-    known[device] = n;
+  int n = known[device].load(std::memory_order_relaxed);
+  if (!n) {
+    if (cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) != cudaSuccess || n <= 0) {
+      (void)cudaGetLastError();
+      n = 148;
+    }
+    known[device].store(n, std::memory_order_relaxed);
   }
-  return known[device];
+  return n;
 }
 
 template <int D, int NG, int NT>

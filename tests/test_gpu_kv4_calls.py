@@ -249,3 +249,29 @@ def test_check_waits_for_calls_on_every_stream():
         cache.check()
     with pytest.raises(cascade_cpp.CascadeError):
         table.check()
+
+
+def test_calls_from_several_threads_on_streams_of_their_own():
+    import threading
+    cache, _ = make(300, 1, 2, 128, 16, 64, seed=9)
+    table = torch.from_numpy(tables(np.random.default_rng(9), [2500, 1300], 300, 16)).to(DEV)
+    lens, start = i32(2500, 1300), i32(0, 90, 92)
+    qs = [torch.randn(92, 8, 128, device=DEV).bfloat16() for _ in range(4)]
+    want = [cache.attend(0, q, table, lens, q_start=start, return_lse=True) for q in qs]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            for _ in range(30):
+                got = cache.attend(0, qs[i], table, lens, q_start=start, return_lse=True)
+                if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                    wrong.append(i)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(qs))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+    cache.check()
