@@ -197,6 +197,13 @@ class KV4Cache(KVPageConnector):
 
     # ------------------------------------------------------------ operators
 
+    def _sizes(self, layer: int, sizes: int) -> None:
+        """Refuses what the C call's 32 bits would wrap (``sizes``: an or of all)."""
+        if not 0 <= layer < self.layers:
+            raise CascadeError(L.CB_ERR_ARG, f"layer must be 0 .. {self.layers - 1}")
+        if sizes >> 31:
+            raise ValueError("sizes must be below 2^31")
+
     def _values(self, t, name: str):
         _on(t, name, self.device)
         if t.dim() != 3 or t.shape[1] != self.kv_heads or t.shape[2] != self.head_dim or (
@@ -216,6 +223,7 @@ class KV4Cache(KVPageConnector):
         if k.dtype != v.dtype or k.shape[0] != v.shape[0]:
             raise ValueError("k and v differ in type or length")
         n = k.shape[0]
+        self._sizes(layer, n)
         at = _vector(slots, "slots", torch.int64, self.device, n)
         _check(_native_lib().cb_kv4_append(
             self._form, layer, _dtype_code(k.dtype), k.data_ptr(), v.data_ptr(), n, k.stride(0), k.stride(1),
@@ -229,6 +237,7 @@ class KV4Cache(KVPageConnector):
         code = _dtype_code(dtype)
         at = _vector(slots, "slots", torch.int64, self.device)
         n = slots.shape[0]
+        self._sizes(layer, n)
         k = torch.empty((n, self.kv_heads, self.head_dim), dtype=dtype, device=self.device)
         v = torch.empty_like(k)
         _check(_native_lib().cb_kv4_read(self._form, layer, code, k.data_ptr(), v.data_ptr(), n, at,
@@ -269,6 +278,7 @@ class KV4Cache(KVPageConnector):
                 block_table.stride(1) != 1 and block_table.shape[1] > 1):
             raise ValueError("block_table must be [requests, columns] with contiguous rows")
         n, columns = block_table.shape
+        self._sizes(layer, rows | heads | n | columns)
         lens = _vector(kv_lens, "kv_lens", torch.int32, dev, n)
         start = None if q_start is None else _vector(q_start, "q_start", torch.int32, dev, n + 1)
         if start is None and rows != n:
@@ -289,7 +299,7 @@ class KV4Cache(KVPageConnector):
             q.data_ptr(), out.data_ptr(), None if lse is None else lse.data_ptr(), block_table.data_ptr(), lens,
             start, None, 0, block_table.stride(0), q.stride(0), q.stride(1),
             d ** -0.5 if scale is None else scale, layer, code, n, columns, rows, heads,
-            (1 if start is None else rows) if max_q is None else max_q, causal, fill)
+            (1 if start is None else rows) if max_q is None else min(max_q, rows), causal, fill)
         lib = _native_lib()
         need = self._work.get((heads, a.max_q))  # the sizes that decide it
         if need is None:
@@ -375,8 +385,8 @@ class PageTable:
                 done = done.view(torch.uint8)
             done = _vector(done, "done", torch.uint8, dev, n)
         tokens = int(tokens)
-        if tokens < 0:
-            raise ValueError("tokens must not be negative")
+        if not 0 <= tokens < 1 << 31:
+            raise ValueError("tokens must be 0 .. 2^31 - 1")
         kv_lens, count = self.kv_lens, self.free_count
         if out is None:  # the int32 outputs share one allocation
             slots = torch.empty(tokens, dtype=torch.int64, device=dev)

@@ -275,3 +275,22 @@ def test_calls_from_several_threads_on_streams_of_their_own():
         t.join()
     assert not wrong
     cache.check()
+
+
+def test_sizes_past_32_bits_are_refused_and_not_wrapped():
+    cache, _ = make(2, 1, 1, 64, 16, 64, seed=9)
+    x = torch.randn(1, 1, 64, device=DEV).half()
+    at, table, lens = torch.tensor([3], device=DEV), torch.zeros(1, 1, dtype=torch.int32, device=DEV), i32(9)
+    before = cache.cache.clone()
+    for layer in (1 << 32, -(1 << 32)):
+        with pytest.raises(cascade_cpp.CascadeError):
+            cache.append(layer, x, x, at)
+        with pytest.raises(cascade_cpp.CascadeError):
+            cache.read(layer, at)
+        with pytest.raises(cascade_cpp.CascadeError):
+            cache.attend(layer, x, table, lens)
+    assert torch.equal(cache.cache, before)
+    want = cache.attend(0, x, table, lens)
+    assert torch.equal(cache.attend(0, x, table, lens, max_q=(1 << 32) + 1), want)
+    with pytest.raises(ValueError):
+        kv4.PageTable(1, 2, 2, 16, device=DEV).plan(i32(1), 1 << 32)
