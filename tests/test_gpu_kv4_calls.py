@@ -294,3 +294,29 @@ def test_sizes_past_32_bits_are_refused_and_not_wrapped():
     assert torch.equal(cache.attend(0, x, table, lens, max_q=(1 << 32) + 1), want)
     with pytest.raises(ValueError):
         kv4.PageTable(1, 2, 2, 16, device=DEV).plan(i32(1), 1 << 32)
+
+
+def test_a_plan_of_many_tokens_is_captured_and_replayed():
+    # the largest cluster, rows that finish and start anew, in a graph
+    rng = np.random.default_rng(6)
+    eager, graph = (kv4.PageTable(300, 20, 4000, 16, device=DEV) for _ in range(2))
+    q, done = torch.zeros(300, dtype=torch.int32, device=DEV), torch.zeros(300, dtype=torch.bool, device=DEV)
+    steps = [(torch.from_numpy(rng.integers(0, 130, 300).astype(np.int32)).to(DEV),
+              torch.from_numpy(rng.random(300) < 0.5).to(DEV)) for _ in range(8)]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        graph.plan(q, 30000, done=done)
+    torch.cuda.current_stream().wait_stream(s)
+    eager.plan(q, 30000, done=done)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = graph.plan(q, 30000, done=done)
+    for a, b in steps:
+        q.copy_(a)
+        done.copy_(b)
+        want = eager.plan(q, 30000, done=done)
+        g.replay()
+        assert all(torch.equal(x, y) for x, y in zip(got, want))
+        assert torch.equal(graph.block_table, eager.block_table)
+    graph.check()

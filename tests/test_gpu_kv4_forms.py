@@ -46,3 +46,14 @@ def test_no_part_of_a_prompt_behind_a_long_prefix_is_lost(dim, group, wide):
 
 def test_single_tokens_beside_drafts_and_chunks():
     held_call("fp16", 128, 64, 16, 2, 4, [500, 33, 410, 90, 0, 260], [1, 5, 60, 1, 0, 16], seed=5)
+
+
+@pytest.mark.parametrize("dim,group,ratio", [(64, 64, 100), (128, 32, 130), (256, 64, 71), (256, 32, 40)])
+def test_more_query_heads_of_a_kv_head_than_a_tile_has_rows(dim, group, ratio):
+    held_call("bf16", dim, group, 16, 1, ratio, [300, 17, 0, 140], [1, 1, 1, 2], seed=ratio)
+
+
+@pytest.mark.parametrize("dim,group,ratio", [(64, 32, 4), (128, 32, 7), (128, 128, 20), (256, 128, 3)])
+def test_a_batch_whose_requests_are_in_a_few_parts_each(dim, group, ratio):
+    lens = [17 * i % 911 + 1 for i in range(1, 61)]
+    held_call("fp16", dim, group, 32, 1, ratio, lens, [1] * len(lens), seed=ratio, max_q=1)
