@@ -16,7 +16,7 @@
 // happens after a row's first tokens, so that O is seldom rescaled.
 //
 // Measured: chunks of 900 to 1,537 tokens behind 5,200 to 9,100 cached ones, 64 / 8
-// heads of 128, bf16: 657 us, 740 TFLOP/s. The tensor cores are busy a third of the
+// heads of 128, bf16: 639 us replayed in a CUDA graph, 761 TFLOP/s. The tensor cores are busy a third of the
 // time, and what stands in their way is shared memory: for two row tiles the products
 // read 192 KB of operands a tile of tokens and the dequantising warps store 64 KB, 2,000
 // cycles of its bandwidth at best; of the 5,000 that a tile takes, a dequantising
@@ -54,12 +54,8 @@ struct PromptLine {
   static constexpr bool kBlock = true;
 };
 
-struct TileFlags {       // of 128 tokens, written by the dequantising warps
-  uint32_t there;        // in each warp's byte: its two cache tiles are there, and kOdd
-  uint32_t pad[3];
-  uint32_t bad_k[4];     // of a warp that set kOdd: a bit for each token whose K is not
-  uint32_t bad_v[4][4];  // finite, and those of V by group
-};
+// What the dequantising warps say of 128 tokens, a byte each: a bit for each of the
+// warp's two cache tiles that is there, and one if a token's K or V is not finite.
 constexpr uint32_t kAllThere = 0x03030303u, kOdd = 0x04040404u;
 
 template <int D, int NG>
@@ -68,7 +64,7 @@ struct PromptForm {
   static constexpr int kOperand = 128 * D * 2;  // bytes of Q, K or V^T
   static constexpr int kQ = 0, kK = 2 * kOperand, kV = 4 * kOperand, kRing = 6 * kOperand;
   static constexpr int kFlags = kRing + kDeqWarps * kRaw * kTile;
-  static constexpr int kBars = kFlags + 4 * (int)sizeof(TileFlags);
+  static constexpr int kBars = kFlags + 16;  // of four tiles
   static constexpr int kSmemUsed = kBars + 256;
   // one block an SM: each takes all of the tensor memory
   static constexpr int kSmem = kSmemUsed > 120 * 1024 ? kSmemUsed : 120 * 1024;
@@ -209,6 +205,34 @@ CB_D __half2 code_high(uint32_t w) {
                  __half2half2(__ushort_as_half(0xd480)));                                             // - 72
 }
 
+// An exponent of all ones in a scale or an offset.
+CB_D bool not_finite(uint32_t par) { return (par & 0x7c00) == 0x7c00 || (par >> 16 & 0x7c00) == 0x7c00; }
+
+// The first tokens of [from, to) that have a V which is not finite, for each group, and a K
+// (first[NG]): a row sees the tokens below its limit, so that the first decides. It reads the
+// pages again, on the way out of an item: with flags of single tokens in the loop over the
+// tiles the prompt chunks named above took 674 us instead of 639. A whole warp calls.
+template <int D, int NG>
+CB_D void first_odd(const Kv4View &c, const AttendArgs &a, const Item &it, int from, int to, int *first) {
+#pragma unroll
+  for (int gi = 0; gi <= NG; ++gi) first[gi] = 0x7fffffff;
+  for (int t = from + (threadIdx.x & 31); t < to; t += 32) {
+    const int page = __ldg(a.block_table + it.b * a.table_stride + (t >> c.page_log2));
+    if (page < 0 || page >= c.num_pages) continue;
+    const uint32_t *p =
+        reinterpret_cast<const uint32_t *>(c.base + (uint64_t)page * c.page_stride + (uint64_t)it.h * c.head_bytes +
+                                           (t & (c.page_size - 1)) / kKv4Tile * (16 * D + 128 * NG) + 16 * D) +
+        t % kKv4Tile * NG;
+#pragma unroll
+    for (int gi = 0; gi < NG; ++gi) {
+      if (not_finite(p[gi])) first[NG] = min(first[NG], t);
+      if (not_finite(p[16 * NG + gi])) first[gi] = min(first[gi], t);
+    }
+  }
+#pragma unroll
+  for (int gi = 0; gi <= NG; ++gi) first[gi] = __reduce_min_sync(0xffffffffu, first[gi]);
+}
+
 // Barriers, 8 bytes each.
 enum {
   kFullK = 0,
@@ -230,7 +254,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
   __shared__ uint32_t tmem_s;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const uint32_t base = smem_addr(smem), bars = base + F::kBars;
-  TileFlags *flags = reinterpret_cast<TileFlags *>(smem + F::kFlags);
+  uint32_t *flags = reinterpret_cast<uint32_t *>(smem + F::kFlags);
   const int most = a.columns * c.page_size, piece = blockIdx.x;
 
   asm volatile("griddepcontrol.launch_dependents;");
@@ -335,13 +359,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
 
         const int limit = row_limit(a, it, min(row, total - 1));
         float l = 0.0f, over = -INFINITY, sub = 0.0f;
-        uint32_t nan_v = 0;  // a bit for each group of which the row sees a V that is not finite
+        uint32_t odd = 0;
         for (int j = 0; j < n && fine; ++j) {
           fine = warp_wait(bars + 8 * (kScores + x), scores_parity);
           scores_parity ^= 1;
           tc_fence_after();
-          const TileFlags &fl = flags[(tile_no + j) & 3];
-          const uint32_t there = fl.there;
+          const uint32_t there = flags[(tile_no + j) & 3];
+          odd |= there;
           const int visible = limit - (w.t0 + j) * kTok;  // columns below it are seen
           const bool masked = __any_sync(0xffffffffu, visible < kTok) || (there & kAllThere) != kAllThere;
           float v[kTok];
@@ -379,17 +403,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
             }
           }
           l *= f;
-          if (there & kOdd) {
-#pragma unroll 1
-            for (int ch = 0; ch < 4; ++ch) {
-              const int left = visible - 32 * ch;
-              const uint32_t sees = left >= 32 ? 0xffffffffu : left > 0 ? (1u << left) - 1 : 0;
-              if (!(there & kOdd & 0xffu << (8 * ch))) continue;
-              if (fl.bad_k[ch] & sees) l = NAN;
-              for (int gi = 0; gi < NG; ++gi)
-                if (fl.bad_v[gi][ch] & sees) nan_v |= 1u << gi;
-            }
-          }
           // ---- weights, P over the columns of S
           const uint64_t by = pair(to_log2, to_log2), minus = pair(-sub, -sub);
           uint64_t sums[2] = {0, 0};
@@ -416,6 +429,14 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
           fine = warp_wait(bars + 8 * (kScores + x), scores_parity);
           scores_parity ^= 1;
           tc_fence_after();
+          uint32_t nan_v = 0;  // a bit for each group of which the row sees a V that is not finite
+          if (odd & kOdd) {
+            int first[NG + 1];
+            first_odd<D, NG>(c, a, it, w.t0 * kTok, min(w.t1 * kTok, it.len), first);
+            if (first[NG] < limit) l = NAN;
+#pragma unroll
+            for (int gi = 0; gi < NG; ++gi) nan_v |= (first[gi] < limit ? 1u : 0u) << gi;
+          }
           const float inv = l == 0.0f ? 0.0f : 1.0f / l;
           const int at_row = x * kTileRows + r;
           float *part = a.parts + ((long long)piece * 2 + (first_segment ? 0 : 1)) * F::kPart;
@@ -542,26 +563,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
         {  // lane: a token
           const uint32_t *kp = reinterpret_cast<const uint32_t *>(ring + (lane < 16 ? stage : next) * F::kTile + 16 * D) +
                                (lane & 15) * NG;
-          auto odd = [](uint32_t p) {  // an exponent of all ones in a scale or an offset
-            return (p & 0x7c00) == 0x7c00 || (p >> 16 & 0x7c00) == 0x7c00;
-          };
-          const bool seen = tok0 + lane < sees_most && (there >> (lane >> 4) & 1);
           bool bad = false;
 #pragma unroll
-          for (int gi = 0; gi < 2 * NG; ++gi) bad |= odd(kp[(gi & 1) * 16 * NG + gi / 2]);
-          const uint32_t votes = __ballot_sync(0xffffffffu, bad && seen);
-          TileFlags &fl = flags[no & 3];
-          if (votes) {
-            bad = false;
-            for (int gi = 0; gi < NG; ++gi) {
-              bad |= odd(kp[gi]);
-              const uint32_t votes_v = __ballot_sync(0xffffffffu, odd(kp[16 * NG + gi]) && seen);
-              if (lane == 0) fl.bad_v[gi][dw] = votes_v;
-            }
-            const uint32_t votes_k = __ballot_sync(0xffffffffu, bad && seen);
-            if (lane == 0) fl.bad_k[dw] = votes_k;
-          }
-          if (lane == 0) reinterpret_cast<uint8_t *>(&fl.there)[dw] = (uint8_t)(there | (votes ? kOdd & 0xffu : 0u));
+          for (int gi = 0; gi < NG; ++gi) bad |= not_finite(kp[gi]) || not_finite(kp[16 * NG + gi]);
+          bad = bad && tok0 + lane < sees_most && (there >> (lane >> 4) & 1);
+          const bool any = __any_sync(0xffffffffu, bad);
+          if (lane == 0)
+            reinterpret_cast<uint8_t *>(flags + (no & 3))[dw] = (uint8_t)(there | (any ? kOdd & 0xffu : 0u));
         }
 #pragma unroll
         for (int ct = 0; ct < 2; ++ct) {
@@ -613,8 +621,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) attend_prompt_kernel(const 
 #pragma unroll
             for (int gi = 0; gi < NG; ++gi) {
               uint32_t p0 = vp[gi], p1 = vp[NG + gi];
-              if (!on0 || (p0 & 0x7c00) == 0x7c00 || (p0 >> 16 & 0x7c00) == 0x7c00) p0 = 0;
-              if (!on1 || (p1 & 0x7c00) == 0x7c00 || (p1 >> 16 & 0x7c00) == 0x7c00) p1 = 0;
+              if (!on0 || not_finite(p0)) p0 = 0;
+              if (!on1 || not_finite(p1)) p1 = 0;
               const __half2 sc = as_half2(__byte_perm(p0, p1, 0x5410)), of = as_half2(__byte_perm(p0, p1, 0x7632));
 #pragma unroll
               for (int j = gi * kGroupWords; j < (gi + 1) * kGroupWords; ++j) {
