@@ -499,7 +499,8 @@ int cb_kv4_read(const cb_kv4_cache *cache, int32_t layer, int32_t dtype, void *k
  * [total_q][q_heads] fp32) or NULL. Rows of no request (before q_start[0], behind
  * q_start[requests]) are left as they were; fill makes them zeros in out
  * (CB_KV4_FILL_OUT) and -inf in lse (CB_KV4_FILL_LSE). max_q is a hint (rows of a
- * request at most); results do not depend on it being right.
+ * request at most), which need not be right: requests of more than 64 rows of a KV
+ * head go to a kernel that rounds K and V to fp16 if it allows for them.
  * workspace: cb_kv4_attend_workspace bytes, 16-byte aligned, used until the
  * call's work is done. */
 typedef struct cb_kv4_attend_args {

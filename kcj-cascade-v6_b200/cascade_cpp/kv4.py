@@ -257,11 +257,15 @@ class KV4Cache(KVPageConnector):
         that sees nothing gets zeros (log-sum-exp -inf). A key that is NaN
         makes the rows that see it NaN, a NaN group of a value its dimensions
         in them. Query heads are in groups of q_heads / kv_heads that share a
-        KV head. ``scale`` defaults to 1 / sqrt(head_dim). ``max_q`` (rows of a request at most) only helps
-        the choice of kernel. Rows of no request (a padded step) are zeros, and
-        left as they were in a given ``out``. With ``return_lse`` also the
-        log-sum-exp of each row's scores, ``[total_q, q_heads]`` fp32, -inf in
-        rows of no request. There is no backward pass."""
+        KV head. ``scale`` defaults to 1 / sqrt(head_dim).
+
+        ``max_q`` (rows of a request at most) only helps the choice of kernel:
+        the one for more than 64 rows of a KV head rounds keys and values to
+        fp16, the one for fewer, which 1 asks for, nothing of the cache. Rows
+        of no request (a padded step) are zeros, and left as they were in a
+        given ``out``. With ``return_lse`` also the log-sum-exp of each row's
+        scores, ``[total_q, q_heads]`` fp32, -inf in rows of no request. There
+        is no backward pass."""
         dev, d = self.device, self.head_dim
         _on(q, "q", dev)
         if q.dim() != 3 or q.shape[2] != d or (q.stride(2) != 1 and q.numel()):

@@ -28,16 +28,19 @@ namespace {
 // exact, with no conversion. Scales and offsets act on 16x8 scores instead of
 // 16xD values: s = scale_k (q.c) + (offset_k - 8 scale_k) sum(q), and V's scale
 // goes into P, p' = p * scale_v, its offset into a sum of p * offset_v - 8 p'.
-// So the only roundings to 16 bits are p' (relative 2^-11; its rounded value
-// is the one that the centring by 8 uses) and the output. q is brought to fp16
-// by a power of two per row: exact for fp16 and, above 2^-28 of the row's
-// largest, for bf16.
+// So the only roundings to 16 bits are p' (relative 2^-11, and 2^-25 of the largest for
+// what is far below it; its rounded value is the one that the centring by 8
+// uses) and the output. For an fp16 output that is an error of 2.4 to 3.1e-4 where
+// the output's rounding alone makes 2.1e-4; the rest of p' as a second operand would
+// take it away for 10 % of the time, and 4-bit values are off by hundreds of
+// times as much. q is brought to fp16 by a power of two per row: exact for fp16 and,
+// above 2^-28 of the row's largest, for bf16 (from 2^111 on it counts as infinite).
 //
 // Bound by HBM where the tokens are many: 1 + 8/group bytes for a cached value pair
-// of K and V. Measured: 48 requests of 9,000 to 32,000 tokens, 64 / 8 heads of 128,
-// group 128: 214 us, 5.0 TB/s; the rest of the way is instructions (266 for a tile
+// of K and V. Measured (replayed in a CUDA graph): 48 requests of 9,000 to 32,000
+// tokens, 64 / 8 heads of 128, group 128: 216 us, 5.0 TB/s; the rest of the way is instructions (266 for a tile
 // of 16 tokens, 16 of them products and 80 the unpacking, at 0.6 an SM quarter and
-// cycle). A single short request is bound by latency: 10.7 us for 1,100 tokens.
+// cycle). A single short request is bound by latency: 10.9 us for 1,100 tokens.
 // mma.sync and not tcgen05: its operands come from registers, where the codes become
 // them with one instruction for two values, and 8 rows leave 15/16 of a 128-row
 // product empty; kv4_prompt.cu has the rows for that.
@@ -823,7 +826,9 @@ auto by_form(int d, int ng, int nt, F f) {
 // one of 8 rows for 16, and costs 3.5 times as much; what several tiles read again is
 // in L2. 24 requests of up to 7,000 tokens, 8 KV heads of 128, us with tiles of 8,
 // 16, 32 rows: 16 rows 54, 52, -; 24 rows 74, 87, 79; 32 rows 91, 89, 84; 40
-// rows 111, 126, 133; 64 rows 166, 163, 139.
+// rows 111, 126, 133; 64 rows 166, 163, 139. (In one group; other forms go by the same
+// rule.) 256 dims in 8 groups take 69 us for 24 such requests of 16 rows, in 4 groups, with
+// tiles of 16 rows, 57.
 int few_tiles(int head_dim, int group, int64_t rows) {
   const int most = most_tiles(head_dim, head_dim / group);
   if (rows <= 8 || most == 1) return 1;
