@@ -71,6 +71,20 @@ def test_a_nan_group_of_v_is_nan_in_its_dims_whatever_its_weight(token, far, hin
 
 
 @pytest.mark.parametrize("hint", [1, None])
+@pytest.mark.parametrize("group", [32, 64])
+def test_a_nan_group_of_v_costs_the_other_groups_of_its_token_nothing(hint, group):
+    cache, ref, table, q = nan_case(40, False, group=group)
+    v = torch.randn(1, 1, 128, device=DEV)
+    v[..., 70] = float("nan")
+    slot = int(table[0, 2]) * 16 + 8
+    cache.append(0, torch.full_like(v, 60.0), v, torch.tensor([slot], device=DEV))  # nearly all the weight
+    ref.data[:] = cache.cache.cpu().numpy()
+    out, lse = cache.attend(0, q, torch.from_numpy(table).to(DEV), i32(200), q_start=i32(0, 100), max_q=hint,
+                            return_lse=True)
+    hold(out, lse, q, ref, 0, table, [200], [100], "fp16", few=hint == 1)
+
+
+@pytest.mark.parametrize("hint", [1, None])
 def test_a_nan_group_of_k_is_nan_in_the_row_and_its_lse(hint):
     cache, ref, table, q = nan_case(198, False, which=0)
     out, lse = cache.attend(0, q, torch.from_numpy(table).to(DEV), i32(200), q_start=i32(0, 100), max_q=hint,
